@@ -9,6 +9,7 @@ models.  Public surface mirrors the reference script's callables:
     onsager_energy …                          onsager.py
     bitflip.BitflipModel / bitflip.diffusion_backward
                                               mnist_diffusion.py: model([X, t]) and its XOR sampler
+    group_norm / adamw_step, AdamW            the norms and the optimizer step of its training
 """
 from .keras_file import UNetSpec, load_unet_spec
 from .onsager import onsager_energy, onsager_heat_capacity, onsager_magnetization, theoretical_critical_kT
@@ -16,7 +17,8 @@ from .onsager import onsager_energy, onsager_heat_capacity, onsager_magnetizatio
 __all__ = ["UNetSpec", "load_unet_spec", "onsager_energy", "onsager_heat_capacity", "onsager_magnetization",
            "theoretical_critical_kT", "load_model", "ScoreModel", "diffusion_backward", "sample", "beta_schedule",
            "observe", "sign_project", "ising_energy", "ising_magnetization", "Observables", "shard_range",
-           "allreduce_observables", "irfft2_sign"]
+           "allreduce_observables", "irfft2_sign",
+           "group_norm", "group_norm_forward", "group_norm_backward", "adamw_state", "adamw_step", "adamw_moments", "AdamW"]
 
 _LAZY = {
     "load_model": "model", "ScoreModel": "model",
@@ -24,6 +26,8 @@ _LAZY = {
     "observe": "observables", "sign_project": "observables", "ising_energy": "observables",
     "ising_magnetization": "observables", "Observables": "observables",
     "irfft2_sign": "spectral",
+    "group_norm": "norm", "group_norm_forward": "norm", "group_norm_backward": "norm",
+    "adamw_state": "optim", "adamw_step": "optim", "adamw_moments": "optim", "AdamW": "optim",
     "shard_range": "distributed", "allreduce_observables": "distributed",
 }
 

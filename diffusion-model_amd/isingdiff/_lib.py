@@ -17,7 +17,7 @@ IDM_UPDATE_SCORE = 0
 IDM_UPDATE_DDPM = 1
 NCONV = 11
 NDENSE = 3
-ABI_VERSION = 3
+ABI_VERSION = 4
 NOALLOC_SCRATCH_BYTES = 64 << 20
 
 
@@ -68,6 +68,23 @@ class MlpDesc(C.Structure):
                 ("w", C.c_void_p * MLP_MAXLAYERS), ("b", C.c_void_p * MLP_MAXLAYERS)]
 
 
+IDM_DT_F32, IDM_DT_BF16, IDM_DT_F16 = 0, 1, 2
+IDM_ACT_NONE, IDM_ACT_SWISH = 0, 1
+ADAMW_BLOCK = 256
+
+
+class GroupNormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("batch", C.c_int64), ("pixels", C.c_int64),
+                ("channels", C.c_int32), ("groups", C.c_int32), ("x_sample", C.c_int64), ("x_pixel", C.c_int64),
+                ("dy_sample", C.c_int64), ("dy_pixel", C.c_int64), ("shift_sample", C.c_int64), ("eps", C.c_float),
+                ("reserved", C.c_int32)]
+
+
+class AdamWCfg(C.Structure):
+    _fields_ = [("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("moment_bits", C.c_int32), ("reserved", C.c_int32),
+                ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double)]
+
+
 # name -> (restype, argtypes); every symbol include/isingdiff.h declares
 SIGNATURES = {
     "idm_abi_version": (C.c_int, []),
@@ -113,6 +130,11 @@ SIGNATURES = {
                                       C.POINTER(C.c_void_p), C.c_void_p]),
     "idm_bitflip_sample": (C.c_int, [C.c_void_p, C.POINTER(BitflipCfg), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                      C.c_int, C.c_int, C.c_void_p]),
+    "idm_group_norm_workspace": (C.c_int, [C.POINTER(GroupNormDesc), C.c_int, C.POINTER(C.c_size_t)]),
+    "idm_group_norm_forward": (C.c_int, [C.c_int, C.POINTER(GroupNormDesc)] + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
+    "idm_group_norm_backward": (C.c_int, [C.c_int, C.POINTER(GroupNormDesc)] + [C.c_void_p] * 12 + [C.c_size_t, C.c_void_p]),
+    "idm_adamw_step": (C.c_int, [C.c_int, C.POINTER(AdamWCfg), C.c_int64] + [C.c_void_p] * 8 + [C.c_int64] + [C.c_void_p] * 3),
+    "idm_adamw_moments": (C.c_int, [C.c_int] + [C.c_void_p] * 6 + [C.c_int64, C.c_void_p]),
 }
 
 _lib = None

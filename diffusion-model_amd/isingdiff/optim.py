@@ -1,0 +1,152 @@
+"""AdamW over many tensors at once, moments in 32 or in 8 bits.
+
+    t += 1;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+    p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+
+Parameters and gradients are float32, bfloat16 or float16 (all parameters of a call of one type, all gradients of one type); the
+arithmetic is float32 and a parameter is rounded once.  The state is a dict of flat tensors: tensor i's moments begin at the sum
+of the sizes before it, each rounded up to 256 entries.
+
+8-bit moments take 1 byte an entry and 2 bytes for each block of 256: a code is a float with three mantissa bits whose
+exponent window (16 binades for m, 32 for v) follows the largest entry of its block.  What is cut off is rounded with a dither that is
+equidistributed over entries and steps, so a second moment that drifts by less than a code a step still moves at its mean rate; an
+entry of m or v is off by up to one code (1/8 of its binade) at any one step.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from .norm import DTYPES
+
+BLOCK = _lib.ADAMW_BLOCK
+
+
+def _room(n: int) -> int:
+    return -(-n // BLOCK) * BLOCK
+
+
+def adamw_state(params, moment_bits: int = 32) -> dict:
+    """The state before the first step: ``step`` int64 (1,) and ``m``, ``v`` on the parameters' device, float32, or uint8 with
+    ``m_base``, ``v_base`` int16 (one per block of 256) for ``moment_bits=8``."""
+    params = list(params)
+    if moment_bits not in (32, 8):
+        raise ValueError("moment_bits must be 32 or 8")
+    if not params:
+        raise ValueError("no parameters")
+    dev, total = params[0].device, sum(_room(p.numel()) for p in params)
+    zeros = lambda n, t: torch.zeros(n, dtype=t, device=dev)  # noqa: E731
+    kind = torch.float32 if moment_bits == 32 else torch.uint8
+    state = {"step": zeros(1, torch.int64), "m": zeros(total, kind), "v": zeros(total, kind)}
+    if moment_bits == 8:
+        state.update(m_base=zeros(total // BLOCK, torch.int16), v_base=zeros(total // BLOCK, torch.int16))
+    return state
+
+
+def _check_state(state, total, dev):
+    """Moment bits of a state that fits `total` entries (None: any whole number of blocks) on `dev`."""
+    eight = state["m"].dtype == torch.uint8
+    kinds = {"step": torch.int64, "m": torch.uint8 if eight else torch.float32, "v": torch.uint8 if eight else torch.float32}
+    if eight:
+        kinds.update(m_base=torch.int16, v_base=torch.int16)
+    total = state["m"].numel() if total is None else total
+    for k, kind in kinds.items():
+        t, n = state[k], 1 if k == "step" else total // BLOCK if k.endswith("base") else total
+        if t.dtype != kind or t.numel() != n or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"state[{k!r}] must be {n} dense {kind} values on {dev}: make it with adamw_state for these parameters")
+    return 8 if eight else 32
+
+
+def _pointers(ts):
+    return (C.c_void_p * len(ts))(*[None if t is None else t.data_ptr() for t in ts])
+
+
+def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01):
+    """One step, in place: ``params``, and ``state`` of :func:`adamw_state`.  ``weight_decay`` is a number, or one per tensor.  A
+    gradient that is None leaves its tensor and moments as they are.  Enqueued on the current stream; a captured step replays with
+    the tensors, lr and decays that it was captured with, while its step count goes on."""
+    params, grads = list(params), list(grads)
+    if not params or len(params) != len(grads):
+        raise ValueError("params and grads must be lists of the same length, not empty")
+    dev, ptype = params[0].device, params[0].dtype
+    gtype = next((g.dtype for g in grads if g is not None), ptype)
+    if ptype not in DTYPES or gtype not in DTYPES:
+        raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
+    sizes = [p.numel() for p in params]
+    for p, g in zip(params, grads):
+        if p.dtype != ptype or p.device != dev or not p.is_contiguous():
+            raise ValueError("parameters must be dense, of one type and on one device")
+        if g is not None and (g.dtype != gtype or g.device != dev or g.shape != p.shape):
+            raise ValueError("a gradient must have its parameter's shape and device, and all gradients one type")
+    grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+    n = len(params)
+    decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+    if len(decay) != n:
+        raise ValueError("weight_decay must be a number or one per tensor")
+    if not (math.isfinite(lr) and lr >= 0 and math.isfinite(eps) and eps >= 0 and all(0 <= b < 1 for b in betas)
+            and all(math.isfinite(w) and w >= 0 for w in decay)):
+        raise ValueError("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)")
+    bits = _check_state(state, sum(_room(s) for s in sizes), dev)
+    if dev.type != "cuda":
+        raise ValueError("parameters must be CUDA tensors")
+    cfg = _lib.AdamWCfg(DTYPES[ptype], DTYPES[gtype], bits, 0, lr, betas[0], betas[1], eps)
+    base = [state[k].data_ptr() if bits == 8 else None for k in ("m_base", "v_base")]
+    with torch.cuda.device(dev):
+        scratch = torch.empty(16, dtype=torch.uint8, device=dev)
+        _lib.check(_lib.load().idm_adamw_step(dev.index, C.byref(cfg), n, _pointers(params), _pointers(grads), (C.c_int64 * n)(*sizes),
+                                              (C.c_float * n)(*decay), state["m"].data_ptr(), state["v"].data_ptr(), *base,
+                                              state["m"].numel(), state["step"].data_ptr(), scratch.data_ptr(),
+                                              torch.cuda.current_stream(dev).cuda_stream))
+    # the kernel writes behind autograd's back: a backward pass that saved a parameter has to see that it changed
+    torch.autograd.graph.increment_version([p for p in params if p.requires_grad])
+
+
+def adamw_moments(state):
+    """The float32 values ``(m, v)`` of a state, flat as its own tensors: those tensors themselves in 32 bits, the values that the codes
+    stand for in 8."""
+    dev = state["m"].device
+    bits = _check_state(state, None, dev)
+    if bits == 32:
+        return state["m"], state["v"]
+    if dev.type != "cuda":
+        raise ValueError("the state must be on a CUDA device")
+    n = state["m"].numel()
+    m, v = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().idm_adamw_moments(dev.index, *(state[k].data_ptr() for k in ("m", "v", "m_base", "v_base")),
+                                                 m.data_ptr(), v.data_ptr(), n, torch.cuda.current_stream(dev).cuda_stream))
+    return m, v
+
+
+class AdamW:
+    """``opt = AdamW(params); loss.backward(); opt.step(); opt.zero_grad()``: :func:`adamw_step` with the gradients that autograd
+    left in ``p.grad``.  ``weight_decay`` may be a number or one per tensor; ``lr`` may be changed between steps."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, moment_bits: int = 32):
+        self.params = list(params)
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.state = adamw_state(self.params, moment_bits)
+
+    def step(self):
+        with torch.no_grad():
+            adamw_step(self.params, [p.grad for p in self.params], self.state, lr=self.lr, betas=self.betas, eps=self.eps,
+                       weight_decay=self.weight_decay)
+
+    def zero_grad(self):
+        for p in self.params:
+            p.grad = None
+
+    def state_dict(self) -> dict:
+        return {k: v.clone() for k, v in self.state.items()}
+
+    def load_state_dict(self, state: dict):
+        if set(state) != set(self.state):
+            raise ValueError("the state has other moments than this optimizer")
+        for k, t in self.state.items():
+            if state[k].shape != t.shape or state[k].dtype != t.dtype:
+                raise ValueError(f"state[{k!r}] does not fit these parameters")
+        for k, t in self.state.items():
+            t.copy_(state[k])

@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define IDM_ABI_VERSION 3
+#define IDM_ABI_VERSION 4
 
 typedef enum {
     IDM_OK = 0,
@@ -343,6 +343,71 @@ int idm_mlp_forward_precision(idm_mlp *m, const float *x_dev, float t_norm, floa
  * traj[T] = x_T and traj[t] = state after step t (the reference's return layout). */
 int idm_mlp_sample(idm_mlp *m, const idm_sample_cfg *cfg, float *x_dev, const float *noise_dev, float *traj_dev,
                    int64_t B, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Operators of training: group normalisation with an activation, forward and backward, and the AdamW step
+ * (the reference trains the same layers through Keras: GroupNormalization + swish, mnist_diffusion/mnist_diffusion.py
+ * :168-193, and keras.optimizers).  They hold no handle and no memory of their own: every buffer, the workspace
+ * included, is the caller's, so calls on different streams with different workspaces are independent, and a call
+ * may be captured into a HIP graph. */
+typedef enum { IDM_DT_F32 = 0, IDM_DT_BF16 = 1, IDM_DT_F16 = 2 } idm_dtype;
+typedef enum { IDM_ACT_NONE = 0, IDM_ACT_SWISH = 1 } idm_activation;
+
+/* x (batch, pixels, channels), channels last, read in place: element (b, p, c) is x[b*x_sample + p*x_pixel + c]; dy likewise
+ * (backward only).  y and dx are dense.  Strides are in elements and not negative; x_pixel, dy_pixel >= channels. */
+typedef struct {
+    int32_t dtype;          /* idm_dtype of x, y, dy, dx */
+    int32_t activation;     /* idm_activation */
+    int64_t batch, pixels;
+    int32_t channels, groups;
+    int64_t x_sample, x_pixel, dy_sample, dy_pixel;
+    int64_t shift_sample;   /* stride of a sample in shift: channels, or 0 when all samples share one row */
+    float eps;              /* forward only */
+    int32_t reserved;
+} idm_group_norm_desc;
+
+/* Bytes of workspace that the forward (backward = 0) or backward call of this shape needs at most.  Launches nothing. */
+int idm_group_norm_workspace(const idm_group_norm_desc *d, int backward, size_t *bytes);
+
+/* u = x + shift[b, c];  xhat = (u - mean) * rstd with mean and rstd = 1 / sqrt(var + eps) over the pixels and channels of a
+ * group;  y = act(xhat * gamma[c] + beta[c]).  gamma, beta, shift: float32, each may be NULL (1, 0, 0).  mean_dev, rstd_dev:
+ * (batch, groups) float32, kept for the backward pass.  Arithmetic is float32; y is rounded once. */
+int idm_group_norm_forward(int device, const idm_group_norm_desc *d, const void *x_dev, const float *gamma_dev,
+                           const float *beta_dev, const float *shift_dev, void *y_dev, float *mean_dev, float *rstd_dev,
+                           void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* Gradients of the above for dy = dL/dy.  dx like y; dgamma, dbeta (channels) and dshift (batch, channels), or (channels) where
+ * shift_sample is 0, float32, each may be NULL.  Sums run in a fixed order: equal inputs give equal bits.  With batch or pixels 0 nothing is written. */
+int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void *dy_dev, const void *x_dev,
+                            const float *mean_dev, const float *rstd_dev, const float *gamma_dev, const float *beta_dev,
+                            const float *shift_dev, void *dx_dev, float *dgamma_dev, float *dbeta_dev, float *dshift_dev,
+                            void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* One AdamW step over n_tensors tensors: t = *step_dev + 1 (written back), and per entry
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * params / grads / sizes / weight_decay: host arrays of n_tensors device pointers, entry counts and decays; a NULL gradient leaves
+ * its tensor and moments as they are.  Gradients and parameters are dense; parameters must not share memory.
+ * Moments: tensor i's begin at the sum of the sizes before it, each rounded up to IDM_ADAMW_BLOCK entries; `moments` is that sum
+ * over all tensors.  moment_bits 32: m_dev, v_dev float32, bases unused.  8: bytes, with one int16 base per block of
+ * IDM_ADAMW_BLOCK entries; code c > 0 stands for the float32 with bits (c + base) << 20 (m: bit 7 is the sign), rounded with a
+ * dither that is equidistributed over entries and steps.  All zero is the state of step 0 in both forms.
+ * scratch_dev: 16 bytes.  The tables are copied at the call: the host arrays may be reused at once, and a captured call replays
+ * with the pointers, lr and decays that it was captured with while the step count goes on. */
+#define IDM_ADAMW_BLOCK 256
+
+typedef struct {
+    int32_t param_dtype, grad_dtype;   /* idm_dtype */
+    int32_t moment_bits, reserved;
+    double lr, beta1, beta2, eps;
+} idm_adamw_cfg;
+
+int idm_adamw_step(int device, const idm_adamw_cfg *cfg, int64_t n_tensors, void *const *params_dev,
+                   const void *const *grads_dev, const int64_t *sizes, const float *weight_decay, void *m_dev, void *v_dev,
+                   int16_t *m_base_dev, int16_t *v_base_dev, int64_t moments, int64_t *step_dev, void *scratch_dev, void *stream);
+
+/* The float32 values that 8-bit moments stand for: `moments` entries each. */
+int idm_adamw_moments(int device, const uint8_t *m_dev, const uint8_t *v_dev, const int16_t *m_base_dev,
+                      const int16_t *v_base_dev, float *m_out_dev, float *v_out_dev, int64_t moments, void *stream);
 
 #ifdef __cplusplus
 }
