@@ -188,11 +188,18 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
 {
     __shared__ float s_mean[THREADS], s_rstd[THREADS];
     const Place w = place_of(g, blockIdx.x, THREADS * V);
-    const int np = g.nchunk * g.tpg;
-    for (int k = threadIdx.x; k < w.ng; k += THREADS) {
+    const int np = g.nchunk * g.tpg, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int k = wave; k < w.ng; k += THREADS / 64) {
         const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
         Moments t = {0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < np; ++i, pp += (int64_t)g.groups * 3) t = join(t, {pp[0], pp[1], pp[2]});
+        for (int i = lane; i < np; i += 64) {
+            const float *o = pp + (int64_t)i * g.groups * 3;
+            t = join(t, {o[0], o[1], o[2]});
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1)
+            t = join(t, {__shfl_xor(t.n, off, 64), __shfl_xor(t.mean, off, 64), __shfl_xor(t.m2, off, 64)});
+        if (lane) continue;
         const float rstd = 1.0f / sqrtf(t.m2 / t.n + g.eps);
         s_mean[k] = t.mean;
         s_rstd[k] = rstd;
@@ -246,6 +253,28 @@ DEVI void grad_z(const float u[V], const float dy[V], const float add[V], float 
     }
 }
 
+// Sums over the rows of buf[rows][width]: done(c, sum) by one thread for each column.  Needs a barrier before and leaves with one.
+template <typename F> DEVI void sum_rows(float *buf, int rows, int width, F &&done)
+{
+    const int TH = (int)blockDim.x, split = TH / width < rows ? TH / width : rows;
+    if (split > 1) {
+        const int c = threadIdx.x % width, s = threadIdx.x / width;
+        float t = 0.0f;
+        if (s < split)
+            for (int k = s; k < rows; k += split) t += buf[k * width + c];
+        __syncthreads();
+        if (s < split) buf[s * width + c] = t;
+        __syncthreads();
+        rows = split;
+    }
+    for (int c = threadIdx.x; c < width; c += TH) {
+        float t = 0.0f;
+        for (int k = 0; k < rows; ++k) t += buf[k * width + c];
+        done(c, t);
+    }
+    __syncthreads();
+}
+
 // Per-channel partial sums of dz, dz * xhat and (for the gradient of shift) xhat: three planes of (batch * nchunk, channels).
 template <typename T, int V, bool SWISH>
 __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const T *__restrict__ dy, const T *__restrict__ x,
@@ -286,16 +315,11 @@ __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const
     }
     const int64_t plane = g.batch * g.nchunk * g.channels, row = (w.b * g.nchunk + w.chunk) * g.channels;
     for (int i = 0; i < (with_xhat ? 3 : 2); ++i) {
-        __syncthreads();
         if (r < rows)
 #pragma unroll
             for (int j = 0; j < V; ++j) sh[(r * q + cq) * V + j] = acc[i][j];
         __syncthreads();
-        for (int c = threadIdx.x; c < w.width; c += THREADS) {
-            float s = 0.0f;
-            for (int k = 0; k < rows; ++k) s += sh[k * w.width + c];
-            sums[i * plane + row + w.c0 + c] = s;
-        }
+        sum_rows(sh, rows, w.width, [&](int c, float s) { sums[i * plane + row + w.c0 + c] = s; });
     }
 }
 
@@ -314,16 +338,13 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
     for (int k = wave; k < w.ng; k += THREADS / 64) {
         const int gc0 = (w.g0 + k) * g.gc;
         float a = 0.0f, b = 0.0f;
-        for (int c = lane; c < g.gc; c += 64) {
-            float t0 = 0.0f, t1 = 0.0f;
-            for (int i = 0; i < g.nchunk; ++i) {
-                const float *o = sb + (int64_t)i * g.channels + gc0 + c;
-                t0 += o[0];
-                t1 += o[plane];
-            }
-            const float gm = g.gamma ? g.gamma[gc0 + c] : 1.0f;
-            a = __builtin_fmaf(gm, t0, a);
-            b = __builtin_fmaf(gm, t1, b);
+#pragma unroll 4
+        for (int64_t e = lane; e < (int64_t)g.nchunk * g.gc; e += 64) {
+            const int64_t i = e / g.gc, c = gc0 + (e - i * g.gc);
+            const float *o = sb + i * g.channels + c;
+            const float gm = g.gamma ? g.gamma[c] : 1.0f;
+            a = __builtin_fmaf(gm, o[0], a);
+            b = __builtin_fmaf(gm, o[plane], b);
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) {
@@ -340,6 +361,7 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
         for (int c = threadIdx.x; c < w.width; c += THREADS) {
             const int ch = w.c0 + c, k = g.tpg == 1 ? c / g.gc : 0;
             float t0 = 0.0f, t2 = 0.0f;
+#pragma unroll 8
             for (int i = 0; i < g.nchunk; ++i) {
                 t0 += sb[(int64_t)i * g.channels + ch];
                 t2 += sb[2 * plane + (int64_t)i * g.channels + ch];
@@ -372,18 +394,444 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
     }
 }
 
-// Column sums of (rows, cols): block (column tile of 64, split s) adds rows s, s + splits, ... to out[s][col].
-__global__ __launch_bounds__(256) void gn_columns_kernel(const float *__restrict__ in, int64_t rows, int cols, int splits,
-                                                         float *__restrict__ out)
+// ---- one launch: a unit (sample, channel tile) held in the registers of one workgroup ---------------------------------
+//
+// Sixteen bytes of a pixel are V consecutive channels; thread (r, cq) holds vector cq of pixels r, r + rows, ... (at most NV).  A
+// vector is cut into P pieces that never straddle a group: P = 1 where a group is whole vectors, 2 where half vectors fit, else
+// V.  x is read once; mean, then the squared distances from it, both over the registers.
+
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+template <typename T> constexpr int vec16 = 16 / (int)sizeof(T);
+
+// The values of a raw vector.  The empty asm keeps the compiler from holding the widened copy between two uses.
+template <typename T> DEVI void widen(u32x4 raw, float out[vec16<T>])
 {
-    __shared__ float sh[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+    asm volatile("" : "+v"(raw));
+    const auto v = __builtin_bit_cast(typename VecOf<T, vec16<T>>::type, raw);
+#pragma unroll
+    for (int j = 0; j < vec16<T>; ++j) out[j] = (float)v[j];
+}
+
+template <typename T> DEVI u32x4 narrow(const float in[vec16<T>])
+{
+    typename VecOf<T, vec16<T>>::type v;
+#pragma unroll
+    for (int j = 0; j < vec16<T>; ++j) v[j] = (T)in[j];
+    return __builtin_bit_cast(u32x4, v);
+}
+
+// A block's memory as a buffer of kNowhere bytes from p on: the plan takes no unit that reaches so far, and a load at kNowhere gives
+// zero, a store there is dropped, so pixels that a thread does not have need no branch.  The whole offset is in the checked
+// (vector) part.
+constexpr int kNowhere = 1 << 30;
+DEVI __amdgpu_buffer_rsrc_t unit_buffer(const void *p, int64_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00020000);
+}
+DEVI u32x4 load16(__amdgpu_buffer_rsrc_t b, int at) { return __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0); }
+DEVI void store16(__amdgpu_buffer_rsrc_t b, int at, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, at, 0, 0); }
+
+// A block is `pack` samples times one tile of ng groups; a sample's part is rows * q threads (`seats`), row r has pixels r, r + rows, ...:
+// full of them, one more where r < more.  Reciprocals instead of divisions: (i + 1/2) * (1 / n) cut to an integer is i / n for the
+// small numbers here (i < 2^13, n <= 2^10: the product is off by less than 2^-10 / n, the nearest integer is 1 / 2n away).
+struct UnitArgs {
+    int64_t batch, x_sample, x_pixel, dy_sample, dy_pixel, shift_sample;
+    int pixels, channels, groups, gc, ng, q, qg, rows, full, more, seats, pack, swish;
+    float inv_q, inv_qg, inv_ng, inv_seats, eps, n, inv_n;   // n: values of a group
+    const float *gamma, *beta, *shift;
+};
+// s / n with r near 1 / n: exact wherever the quotient is a float (a constant group's mean is its value)
+DEVI float over(float s, float n, float r)
+{
+    const float m = s * r;
+    return __builtin_fmaf(__builtin_fmaf(-m, n, s), r, m);
+}
+DEVI int quotient(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
+
+constexpr int kTileVecs = 64;   // vectors of a tile, unless one group (or the fewest whole groups that are whole vectors) is wider
+
+// V consecutive float32 from a 16-byte aligned place
+template <int V> DEVI void load_chan16(const float *p, int c, float missing, float out[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const f32x4 v = p ? *(const f32x4 *)(p + c + i) : f32x4{missing, missing, missing, missing};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[i + j] = v[j];
+    }
+}
+
+// sum += the vector's values, squares += their squares, both in float32 from pairs
+DEVI void add_pairs(u32x4 raw, _Float16, float &sum, float &squares)
+{
+    typedef __attribute__((ext_vector_type(2))) _Float16 half2_;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned w = raw[j];   // (a copy: the cast of an element itself takes the first one)
+        const half2_ v = __builtin_bit_cast(half2_, w);
+        sum = __builtin_amdgcn_fdot2(v, half2_{1, 1}, sum, false);
+        squares = __builtin_amdgcn_fdot2(v, v, squares, false);
+    }
+}
+DEVI void add_pairs(u32x4 raw, __bf16, float &sum, float &squares)
+{
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned w = raw[j];
+        const bf2 v = __builtin_bit_cast(bf2, w);
+        sum = __builtin_amdgcn_fdot2_f32_bf16(v, bf2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+        squares = __builtin_amdgcn_fdot2_f32_bf16(v, v, squares, false);
+    }
+}
+
+struct Seat {
+    int64_t b;                 // sample
+    int sub, r, cq, c, mine;   // sample of the pack, row, vector of the row, its first channel, pixels
+    bool active;
+};
+template <int V> DEVI Seat seat_of(const UnitArgs &g, int64_t pack, int tile)
+{
+    Seat s;
+    s.sub = quotient(threadIdx.x, g.inv_seats);
+    const int l = threadIdx.x - s.sub * g.seats;
+    s.r = quotient(l, g.inv_q);
+    s.cq = l - s.r * g.q;
+    s.c = (tile * g.q + s.cq) * V;
+    s.b = pack * g.pack + s.sub;
+    s.active = s.sub < g.pack && s.b < g.batch;
+    s.mine = s.active ? g.full + (s.r < g.more) : 0;
+    return s;
+}
+
+// Joins the pieces of each group of the block: `lanes` (a power of two) lanes take one group together.  load(entry of part, row) and
+// add work on a lane's running value, done(sub, group of the tile, value) runs on one lane of each group.  Pieces of a group are qg
+// consecutive ones of each row of `row` pieces.
+template <typename A, typename B, typename C> DEVI void fold_groups(const UnitArgs &g, int P, A &&first, B &&second, C &&done)
+{
+    const int entries = g.rows * g.qg, row = g.q * P, all = g.pack * g.ng;
+    int lanes = 1;
+    while (lanes < 64 && lanes < entries) lanes <<= 1;
+    const int lane = threadIdx.x & (lanes - 1), step = (int)blockDim.x / lanes;
+    for (int k0 = 0; k0 < all; k0 += step) {
+        const int k = k0 + (int)threadIdx.x / lanes, sub = quotient(k, g.inv_ng), grp = k - sub * g.ng;
+        const bool on = k < all;
+        const int base = sub * g.seats * P + grp * g.qg;
+        auto sum = [&](auto &&term) {
+            float2 t = {0.0f, 0.0f};
+            if (on)
+                for (int e = lane; e < entries; e += lanes) {
+                    const int r = quotient(e, g.inv_qg);
+                    term(t, base + r * row + e - r * g.qg, r);
+                }
+            for (int w = lanes >> 1; w >= 1; w >>= 1) {
+                t.x += __shfl_xor(t.x, w, 64);
+                t.y += __shfl_xor(t.y, w, 64);
+            }
+            return t;
+        };
+        const float2 a = sum(first);
+        const float2 b = second(a, sum);
+        if (on && lane == 0) done(sub, grp, k, b);
+    }
+}
+
+// Grid: x samples (or packs) that are neighbours, y tiles, z the next ones.  Consecutive blocks go to the eight dies in turn, so
+// x = 8 keeps the tiles of one sample on one die, whose cache joins their parts of a line.
+template <typename T, int P, int TH, int NV>
+__global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T *__restrict__ x, T *__restrict__ y,
+                                                             float *__restrict__ mean_out, float *__restrict__ rstd_out)
+{
+    constexpr int V = vec16<T>, PS = V / P, E = sizeof(T);
+    extern __shared__ float lds[];
+    float2 *const part = (float2 *)lds, *const stat = part + blockDim.x * P;
+    const int64_t pack = (int64_t)blockIdx.z * gridDim.x + blockIdx.x, b0 = pack * g.pack;
+    if (b0 >= g.batch) return;
+    const Seat s = seat_of<V>(g, pack, blockIdx.y);
+    const int c0 = blockIdx.y * g.q * V;
+    u32x4 raw[NV];
+    {
+        const auto xb = unit_buffer(x + b0 * g.x_sample + c0, kNowhere);
+        const int pitch = (int)g.x_pixel * E, at = (int)(s.sub * g.x_sample) * E + s.r * pitch + s.cq * 16;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) raw[k] = load16(xb, k < s.mine ? at + k * g.rows * pitch : kNowhere);
+    }
+    float add[V], mean[P], m2[P];
+    load_chan16<V>(g.shift && s.active ? g.shift + s.b * g.shift_sample : nullptr, s.c, 0.0f, add);
+    // The thread's own mean and squared distances from it, then the group's from all of its threads'.  A sum of squares around zero
+    // would lose the variance of values far from it, so the distances are summed; only where 16-bit values come without a shift,
+    // and the thread's mean turns out to be within four of its deviations, do sum and sum of squares (two instructions for two
+    // values instead of eight) stand: that loses less than five bits.
+    const float own = (float)(s.mine ? s.mine * PS : 1), share = __builtin_amdgcn_rcpf(own);
+    bool sure = false;
+    if constexpr (E == 2 && P == 1) {
+        if (!g.shift) {
+            float sum = 0.0f, squares = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) add_pairs(raw[k], T{}, sum, squares);
+            mean[0] = over(sum, own, share);
+            m2[0] = squares - sum * mean[0];
+            sure = !(m2[0] * 16.0f < sum * mean[0]);
+        }
+    }
+    if (!sure) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            mean[i] = m2[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PS; ++j) mean[i] += add[i * PS + j];
+            mean[i] *= (float)s.mine;
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float v[V];
+            widen<T>(raw[k], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) mean[j / PS] += v[j];
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) mean[i] = over(mean[i], own, share);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (k >= s.mine) continue;
+            float v[V];
+            widen<T>(raw[k], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = v[j] + (add[j] - mean[j / PS]);
+                m2[j / PS] = __builtin_fmaf(d, d, m2[j / PS]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) part[threadIdx.x * P + i] = float2{mean[i], m2[i]};
+    __syncthreads();
+    const auto count = [&](int r) { return (float)((g.full + (r < g.more)) * PS); };
+    fold_groups(
+        g, P, [&](float2 &t, int at, int r) { t.x = __builtin_fmaf(count(r), part[at].x, t.x); },
+        [&](float2 sum, auto &&again) {
+            const float m = over(sum.x, g.n, g.inv_n);
+            const float2 d2 = again([&](float2 &t, int at, int r) {
+                const float2 o = part[at];
+                const float d = o.x - m;
+                t.x += __builtin_fmaf(count(r) * d, d, o.y);
+            });
+            return float2{m, 1.0f / sqrtf(d2.x * g.inv_n + g.eps)};
+        },
+        [&](int sub, int grp, int k, float2 v) {
+            stat[k] = v;
+            if (b0 + sub < g.batch) {
+                const int64_t o = (b0 + sub) * g.groups + blockIdx.y * g.ng + grp;
+                mean_out[o] = v.x;
+                rstd_out[o] = v.y;
+            }
+        });
+    __syncthreads();
+    // z = (x + add) * a + sh in float32; 16-bit values, which cannot lie far from zero in units of what they resolve, take add * a
+    // into sh (its rounding is 2^-24 of |mean| / deviation, theirs 2^-9 or 2^-12 of the value)
+    float a[V], sh[V];
+    load_chan16<V>(s.active ? g.gamma : nullptr, s.c, 1.0f, a);
+    load_chan16<V>(s.active ? g.beta : nullptr, s.c, 0.0f, sh);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const float2 t = stat[s.active ? s.sub * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0];
+#pragma unroll
+        for (int j = i * PS; j < (i + 1) * PS; ++j) {
+            add[j] -= t.x;
+            a[j] *= t.y;
+            if constexpr (E == 2) sh[j] = __builtin_fmaf(add[j], a[j], sh[j]);
+        }
+    }
+    const int pitch = g.channels * E, at = (s.sub * g.pixels + s.r) * pitch + s.cq * 16;
+    const auto yb = unit_buffer(y + b0 * g.pixels * g.channels + c0, kNowhere);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        float v[V];
+        widen<T>(raw[k], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(E == 2 ? v[j] : v[j] + add[j], a[j], sh[j]);
+        if (g.swish)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] *= sigmoid(v[j]);
+        store16(yb, k < s.mine ? at + k * g.rows * pitch : kNowhere, narrow<T>(v));
+    }
+}
+
+// Backward of a unit: x and dy are read once; dz stays in the registers in float32 between the group sums and dx.  A block walks
+// over packs `walker`, walker + walkers, ... of one tile and keeps the tile's weight gradients (in LDS, a thread's own sums); it
+// writes them once, as row `walker` of two planes (walkers, channels).
+template <typename T, int P, int TH, int NV>
+__global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : sizeof(T) == 4 ? 4 : 3) void gn_unit_backward_kernel(
+    UnitArgs g, int walkers, const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ mean_in,
+    const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ sums, float *__restrict__ dshift)
+{
+    constexpr int V = vec16<T>, PS = V / P, E = sizeof(T);
+    extern __shared__ float lds[];
+    float *const total[2] = {lds, lds + blockDim.x * V}, *const buf = lds + 2 * blockDim.x * V;
+    float2 *const part = (float2 *)buf, *const stat = (float2 *)(buf + blockDim.x * (V > 2 * P ? V : 2 * P));
+    const int walker = blockIdx.z * gridDim.x + blockIdx.x;
+    if (walker >= walkers) return;
+    const int width = g.q * V, c0 = blockIdx.y * width;
+    const int xpitch = (int)g.x_pixel * E, dpitch = (int)g.dy_pixel * E, opitch = g.channels * E;
+#pragma unroll
+    for (int j = 0; j < V; ++j) total[0][threadIdx.x * V + j] = total[1][threadIdx.x * V + j] = 0.0f;
+    for (int64_t pack = walker; pack * g.pack < g.batch; pack += walkers) {
+        const Seat s = seat_of<V>(g, pack, blockIdx.y);
+        const int64_t b0 = pack * g.pack;
+        u32x4 raw[NV], up[NV];
+        {
+            const auto xb = unit_buffer(x + b0 * g.x_sample + c0, kNowhere), db = unit_buffer(dy + b0 * g.dy_sample + c0, kNowhere);
+            const int xat = (int)(s.sub * g.x_sample) * E + s.r * xpitch + s.cq * 16, dat = (int)(s.sub * g.dy_sample) * E + s.r * dpitch + s.cq * 16;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                raw[k] = load16(xb, k < s.mine ? xat + k * g.rows * xpitch : kNowhere);
+                up[k] = load16(db, k < s.mine ? dat + k * g.rows * dpitch : kNowhere);
+            }
+        }
+        // u = x + add (float32) or x (16 bits), xhat = u * rstd + off, z = u * a + sh.  The loop sums dz and dz * u; dz * xhat
+        // follows from them.
+        float add[V], off[V], rstd[P], a[V], sh[V];
+        load_chan16<V>(g.shift && s.active ? g.shift + s.b * g.shift_sample : nullptr, s.c, 0.0f, add);
+        load_chan16<V>(s.active ? g.gamma : nullptr, s.c, 1.0f, a);
+        load_chan16<V>(s.active ? g.beta : nullptr, s.c, 0.0f, sh);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int64_t at = s.active ? s.b * g.groups + blockIdx.y * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0;
+            const float mean = mean_in[at];
+            rstd[i] = rstd_in[at];
+#pragma unroll
+            for (int j = i * PS; j < (i + 1) * PS; ++j) {
+                add[j] -= mean;
+                off[j] = E == 2 ? add[j] * rstd[i] : 0.0f;
+                sh[j] = __builtin_fmaf(off[j], a[j], sh[j]);
+                a[j] *= rstd[i];
+            }
+        }
+        float dz[NV][V], s0[V], s1[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (k >= s.mine) continue;
+            float u[V];
+            widen<T>(raw[k], u);
+            widen<T>(up[k], dz[k]);
+            if constexpr (E == 4)
+#pragma unroll
+                for (int j = 0; j < V; ++j) u[j] += add[j];
+            if (g.swish)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float z = __builtin_fmaf(u[j], a[j], sh[j]), sg = sigmoid(z);
+                    dz[k][j] *= __builtin_fmaf(z * sg, 1.0f - sg, sg);
+                }
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                s0[j] += dz[k][j];
+                s1[j] = __builtin_fmaf(dz[k][j], u[j], s1[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) s1[j] = __builtin_fmaf(s1[j], rstd[j / PS], off[j] * s0[j]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {   // gamma * dz and gamma * dz * xhat, times rstd
+            float2 t = {0.0f, 0.0f};
+#pragma unroll
+            for (int j = i * PS; j < (i + 1) * PS; ++j) {
+                t.x = __builtin_fmaf(a[j], s0[j], t.x);
+                t.y = __builtin_fmaf(a[j], s1[j], t.y);
+            }
+            part[threadIdx.x * P + i] = t;
+        }
+        if (s.active)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                total[0][threadIdx.x * V + j] += s0[j];
+                total[1][threadIdx.x * V + j] += s1[j];
+            }
+        __syncthreads();
+        fold_groups(
+            g, P,
+            [&](float2 &t, int at, int) {
+                const float2 o = part[at];
+                t.x += o.x;
+                t.y += o.y;
+            },
+            [&](float2 t, auto &&) { return float2{t.x * g.inv_n, t.y * g.inv_n}; },
+            [&](int, int, int k, float2 v) { stat[k] = v; });
+        __syncthreads();
+        // dx = dz * a - (A + B * xhat) with rstd in A and B: dz * a + u * cx + c0
+        float cx[P], c0v[V];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const float2 t = stat[s.active ? s.sub * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0];
+            cx[i] = -rstd[i] * t.y;
+#pragma unroll
+            for (int j = i * PS; j < (i + 1) * PS; ++j) c0v[j] = -__builtin_fmaf(off[j], t.y, t.x);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) s0[j] = 0.0f;
+        const auto ob = unit_buffer(dx + b0 * g.pixels * g.channels + c0, kNowhere);
+        const int oat = (s.sub * g.pixels + s.r) * opitch + s.cq * 16;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (k >= s.mine) continue;
+            float u[V];
+            widen<T>(raw[k], u);
+#pragma unroll
+            for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(dz[k][j], a[j], __builtin_fmaf(E == 2 ? u[j] : u[j] + add[j], cx[j / PS], c0v[j]));
+            if (dshift)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s0[j] += u[j];
+            store16(ob, oat + k * g.rows * opitch, narrow<T>(u));
+        }
+        if (dshift) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) buf[threadIdx.x * V + j] = s0[j];
+            __syncthreads();
+            if (g.pack == 1) {
+                sum_rows(buf, g.rows, width, [&](int k, float t) { dshift[b0 * g.channels + c0 + k] = t; });
+            } else {   // few rows each
+                for (int i = threadIdx.x; i < g.pack * width; i += blockDim.x) {
+                    const int sub = i / width, k = i - sub * width;
+                    float t = 0.0f;
+                    for (int r = 0; r < g.rows; ++r) t += buf[(sub * g.rows + r) * width + k];
+                    if (b0 + sub < g.batch) dshift[(b0 + sub) * g.channels + c0 + k] = t;
+                }
+                __syncthreads();
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = 0; i < 2; ++i)
+        sum_rows(total[i], g.rows * g.pack, width, [&](int k, float t) { sums[((int64_t)i * walkers + walker) * g.channels + c0 + k] = t; });
+}
+
+// Column sums of planes (rows, cols): block (16 columns, plane, split) adds rows split, split + splits, ...
+__global__ __launch_bounds__(256) void gn_columns_kernel(const float *__restrict__ in, int64_t rows, int cols, int splits, float *__restrict__ out0,
+                                                         float *__restrict__ out1)
+{
+    __shared__ float sh[16][17];
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, col = blockIdx.x * 16 + lane;
+    const float *p = in + (int64_t)blockIdx.y * rows * cols + col;
+    float *out = blockIdx.y ? out1 : out0;
     float s = 0.0f;
     if (col < cols)
-        for (int64_t r = blockIdx.y + (int64_t)wave * splits; r < rows; r += 4 * (int64_t)splits) s += in[r * cols + col];
-    sh[wave][lane] = s;
+#pragma unroll 8
+        for (int64_t r = blockIdx.z + (int64_t)row * splits; r < rows; r += 16 * (int64_t)splits) s += p[r * cols];
+    sh[row][lane] = s;
     __syncthreads();
-    if (wave == 0 && col < cols) out[(int64_t)blockIdx.y * cols + col] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+    if (row == 0 && col < cols && out) {
+        float t[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t[k] = sh[k][lane];
+#pragma unroll
+        for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; ++k) t[k] += t[k + w];
+        out[(int64_t)blockIdx.z * cols + col] = t[0];
+    }
 }
 
 constexpr int kSplits = 64;
@@ -430,18 +878,179 @@ Geometry geometry_of(const idm_group_norm_desc &d, int v)
     return g;
 }
 
-// The vector width depends on pointers, which the size query does not have: the smallest tiles (V = 1) and most chunks bound it.
+// Column sums of one plane (out1 null) or two; part: 2 * kSplits * cols floats
+void column_sums(const float *in, int64_t rows, int cols, float *part, float *out0, float *out1, int planes, hipStream_t s)
+{
+    const unsigned ct = (unsigned)((cols + 15) / 16);
+    const int splits = rows > 2048 ? kSplits : 1;
+    if (splits > 1) {
+        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, planes, splits), dim3(256), 0, s, in, rows, cols, splits, part, part + (size_t)kSplits * cols);
+        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, planes, 1), dim3(256), 0, s, (const float *)part, (int64_t)splits, cols, 1, out0, out1);
+    } else {
+        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, planes, 1), dim3(256), 0, s, in, rows, cols, 1, out0, out1);
+    }
+}
+
+// ---- the one-launch form: which calls take it, with which instance and tile
+struct UnitPlan {
+    int pieces, threads, nv, tiles, ng, q, rows, pack;
+    int64_t walkers;    // backward: blocks that share the samples of a tile
+};
+
+struct Instance { int threads, nv; };            // most threads, vectors of a thread
+constexpr Instance kForward[] = {{1024, 8}, {1024, 16}, {1024, 4}};
+constexpr Instance kBackward[] = {{512, 8}, {768, 4}};
+
+// Does not look at pointers: `aligned` says whether they are 16-byte aligned.
+bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPlan &u)
+{
+    const int e = elem_bytes(d.dtype), v = 16 / e, gc = d.channels / d.groups;
+    if (!aligned || d.channels % v || d.shift_sample % 4 || d.x_sample % v || d.x_pixel % v || (backward && (d.dy_sample % v || d.dy_pixel % v))) return false;
+    const int64_t pitch = std::max<int64_t>({d.x_pixel, d.channels, backward ? d.dy_pixel : 0});
+    const int64_t apart = std::max<int64_t>({d.x_sample, d.pixels * d.channels, backward ? d.dy_sample : 0});
+    if (d.pixels > 1024 * 16 || d.pixels * pitch * e >= kNowhere / 2) return false;
+    u = {};
+    u.pieces = gc % v == 0 ? 1 : gc % (v / 2) == 0 ? 2 : v;
+    int whole = 1;                                   // fewest groups that are whole vectors
+    while (whole * gc % v) ++whole;
+    const int wide = whole * gc / v, units = d.groups / whole;
+    const Instance *list = backward ? kBackward : kForward;
+    auto fits = [&](int tiles, int i) {
+        if (units % tiles) return false;
+        const int t = units / tiles, q = t * wide;
+        if (q > kTileVecs && t > 1) return false;
+        const int64_t rows = (d.pixels + list[i].nv - 1) / list[i].nv, seats = rows * q;
+        if (seats > list[i].threads) return false;
+        // small maps: several samples to a block, of a wavefront's work at least
+        int64_t pack = std::max<int64_t>(1, std::min<int64_t>(128 / seats, d.batch * tiles / 1024));
+        if (pack * apart * e >= kNowhere / 2) pack = 1;
+        u.threads = (int)((seats * pack + 63) / 64 * 64);
+        u.nv = list[i].nv;
+        u.ng = t * whole;
+        u.tiles = tiles;
+        u.q = q;
+        u.rows = (int)rows;
+        u.pack = (int)pack;
+        return true;
+    };
+    auto walkers = [&](int64_t want) {
+        const int64_t packs = (d.batch + u.pack - 1) / u.pack, turns = (packs + want - 1) / want;
+        u.walkers = (packs + turns - 1) / turns;
+        return true;
+    };
+    bool ok = false;
+    // The narrowest tile of whole 64-byte parts that makes 256 blocks: narrow ones leave several blocks to a compute unit, one of which
+    // loads while another computes; parts of 48 or 32 bytes cost a third of the bandwidth (1 024 x 28 x 28 x 96 bf16, forward: tiles of
+    // 32 / 64 / 96 / 192 bytes 85 / 67 / 75 / 75 us).  With fewer samples the chip fills first: narrower tiles.
+    for (int i = 0; i < (backward ? 1 : 2) && !ok; ++i)
+        for (int tiles = units; tiles >= 1 && !ok; --tiles) ok = units % tiles == 0 && units / tiles * wide % 4 == 0 && d.batch * tiles >= 256 && fits(tiles, i);
+    for (int i = 0; i < 2 && !ok; ++i)
+        for (int tiles = 1; tiles <= units && !ok; ++tiles) ok = d.batch * tiles >= 256 && fits(tiles, i);
+    for (int i = 0; i < 2 && !ok; ++i) ok = fits(units, i) && (u.threads <= 512 || d.batch * units >= 128);
+    if (!ok) return false;
+    return walkers((256 * 1024 / u.threads + u.tiles - 1) / u.tiles);
+}
+
+// What a call needs.  Unless the caller says that all pointers are aligned, the size query does not know which form and vector width
+// the call will take: the largest of all.
 size_t workspace_floats(const idm_group_norm_desc &d, bool backward)
 {
-    size_t most = 0;
-    for (int v = 16 / elem_bytes(d.dtype); v >= 1; v >>= 1) {
-        if ((d.channels / d.groups) % v) continue;
-        const Geometry g = geometry_of(d, v);
-        const size_t rows = (size_t)g.batch * g.nchunk;
-        most = std::max(most, backward ? 3 * rows * g.channels : rows * g.tpg * g.groups * 3);
-    }
-    if (backward) most += (size_t)kSplits * d.channels + (d.shift_sample == 0 ? (size_t)d.batch * d.channels : 0);
+    UnitPlan u;
+    const bool unit = plan_unit(d, backward, true, u);
+    size_t most = unit && backward ? (size_t)2 * u.walkers * d.channels : 0;
+    if (!(unit && d.aligned))
+        for (int v = 16 / elem_bytes(d.dtype); v >= 1; v >>= 1) {
+            if ((d.channels / d.groups) % v) continue;
+            const Geometry g = geometry_of(d, v);
+            const size_t rows = (size_t)g.batch * g.nchunk;
+            most = std::max(most, backward ? 3 * rows * g.channels : rows * g.tpg * g.groups * 3);
+        }
+    if (backward) most += (size_t)2 * kSplits * d.channels + (d.shift_sample == 0 ? (size_t)d.batch * d.channels : 0);
     return most;
+}
+
+UnitArgs unit_args(const idm_group_norm_desc &d, const UnitPlan &u)
+{
+    UnitArgs a = {};
+    a.batch = d.batch; a.x_sample = d.x_sample; a.x_pixel = d.x_pixel; a.dy_sample = d.dy_sample; a.dy_pixel = d.dy_pixel;
+    a.shift_sample = d.shift_sample; a.pixels = (int)d.pixels; a.channels = d.channels; a.groups = d.groups;
+    a.gc = d.channels / d.groups; a.swish = d.activation == IDM_ACT_SWISH;
+    a.ng = u.ng; a.q = u.q; a.rows = u.rows; a.pack = u.pack; a.seats = u.rows * u.q;
+    a.qg = u.q * u.pieces / u.ng;
+    a.full = a.pixels / u.rows; a.more = a.pixels % u.rows;
+    a.inv_q = 1.0f / (float)a.q; a.inv_qg = 1.0f / (float)a.qg; a.inv_ng = 1.0f / (float)a.ng; a.inv_seats = 1.0f / (float)a.seats;
+    a.eps = d.eps; a.n = (float)d.pixels * (float)a.gc; a.inv_n = 1.0f / a.n;
+    return a;
+}
+
+constexpr int64_t kGridZ = 65535;
+
+// n samples (or packs, or walkers) in a grid: eight neighbours in x where there are enough of them
+dim3 unit_grid(int64_t n, int tiles)
+{
+    const unsigned x = n >= 64 ? 8 : (unsigned)n;
+    return dim3(x, tiles, (unsigned)((n + x - 1) / x));
+}
+
+template <typename T, int P>
+int unit_forward(const UnitPlan &u, UnitArgs a, const void *x, void *y, float *mean, float *rstd, hipStream_t s)
+{
+    const size_t lds = ((size_t)u.threads * P + (size_t)u.pack * u.ng) * sizeof(float2);
+    const int64_t most = kGridZ * 8 * u.pack, all = a.batch;   // samples of one launch
+    for (int64_t b = 0; b < all; b += most) {
+        a.batch = std::min(most, all - b);
+        const dim3 grid = unit_grid((a.batch + u.pack - 1) / u.pack, u.tiles);
+        const T *xb = (const T *)x + b * a.x_sample;
+        T *yb = (T *)y + b * a.pixels * a.channels;
+        UnitArgs ab = a;
+        if (ab.shift) ab.shift += b * a.shift_sample;
+#define IDM_GN_UNIT(TH, NV)                                                                                                       \
+    if (u.nv == NV)                                                                                                               \
+        hipLaunchKernelGGL((gn_unit_forward_kernel<T, P, TH, NV>), grid, dim3(u.threads), lds, s, ab, xb, yb, mean + b * a.groups, \
+                           rstd + b * a.groups)
+        IDM_GN_UNIT(1024, 4); else IDM_GN_UNIT(1024, 8); else IDM_GN_UNIT(1024, 16);
+#undef IDM_GN_UNIT
+    }
+    return hipGetLastError() == hipSuccess ? IDM_OK : idm_set_error(IDM_ERR_HIP, "group norm: launch failed");
+}
+
+template <typename T, int P>
+int unit_backward(const UnitPlan &u, const UnitArgs &a, const void *dy, const void *x, const float *mean, const float *rstd, void *dx,
+                  float *dgamma, float *dbeta, float *dshift, float *ws, hipStream_t s)
+{
+    const size_t lds = (size_t)u.threads * (2 * vec16<T> + std::max(vec16<T>, 2 * P)) * sizeof(float) + (size_t)u.pack * u.ng * sizeof(float2);
+    float *part = ws + 2 * u.walkers * a.channels, *rows = dshift;
+    if (dshift && a.shift_sample == 0) rows = part + (size_t)2 * kSplits * a.channels;   // one row for all samples: summed below
+#define IDM_GN_UNIT(TH, NV)                                                                                                         \
+    if (u.nv == NV)                                                                                                                 \
+        hipLaunchKernelGGL((gn_unit_backward_kernel<T, P, TH, NV>), unit_grid(u.walkers, u.tiles), dim3(u.threads), lds, s, a,          \
+                           (int)u.walkers, (const T *)dy, (const T *)x, mean, rstd, (T *)dx, ws, rows)
+    IDM_GN_UNIT(768, 4); else IDM_GN_UNIT(512, 8);
+#undef IDM_GN_UNIT
+    if (dbeta || dgamma) column_sums(ws, u.walkers, a.channels, part, dbeta, dgamma, 2, s);
+    if (rows != dshift) column_sums(rows, a.batch, a.channels, part, dshift, nullptr, 1, s);
+    return hipGetLastError() == hipSuccess ? IDM_OK : idm_set_error(IDM_ERR_HIP, "group norm backward: launch failed");
+}
+
+template <typename F> int by_piece(int dtype, int pieces, F &&f)
+{
+    auto go = [&](auto t) {
+        constexpr int V = vec16<decltype(t)>;
+        return pieces == 1 ? f(t, std::integral_constant<int, 1>{}) : pieces == 2 ? f(t, std::integral_constant<int, 2>{})
+                                                                                  : f(t, std::integral_constant<int, V>{});
+    };
+    switch (dtype) {
+    case IDM_DT_F32: return go(float{});
+    case IDM_DT_BF16: return go(__bf16{});
+    default: return go(_Float16{});
+    }
+}
+
+bool aligned16(std::initializer_list<const void *> ptrs)
+{
+    for (const void *p : ptrs)
+        if ((uintptr_t)p % 16) return false;
+    return true;
 }
 
 int check_desc(const idm_group_norm_desc *d, bool backward)
@@ -482,19 +1091,6 @@ int forward_launch(const idm_group_norm_desc &d, const Geometry &g, const void *
     return check_launch("group norm: launch failed");
 }
 
-// out[c] = sum of column c of (rows, cols); part: kSplits * cols floats
-void column_sums(const float *in, int64_t rows, int cols, float *part, float *out, hipStream_t s)
-{
-    const unsigned ct = (unsigned)((cols + 63) / 64);
-    const int splits = (int)std::min<int64_t>(kSplits, (rows + 15) / 16);
-    if (splits > 1) {
-        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, (unsigned)splits), dim3(256), 0, s, in, rows, cols, splits, part);
-        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, 1), dim3(256), 0, s, (const float *)part, (int64_t)splits, cols, 1, out);
-    } else {
-        hipLaunchKernelGGL(gn_columns_kernel, dim3(ct, 1), dim3(256), 0, s, in, rows, cols, 1, out);
-    }
-}
-
 template <typename T, int V, bool SWISH>
 int backward_launch(const Geometry &g, const void *dy, const void *x, const float *mean, const float *rstd, void *dx, float *dgamma,
                     float *dbeta, float *dshift, float *ws, hipStream_t s)
@@ -504,12 +1100,11 @@ int backward_launch(const Geometry &g, const void *dy, const void *x, const floa
     hipLaunchKernelGGL((gn_grad_sums_kernel<T, V, SWISH>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)dy, (const T *)x, mean,
                        rstd, ws, dshift != nullptr);
     float *part = ws + 3 * plane, *per_sample = nullptr;
-    if (dshift && g.shift_sample == 0) per_sample = part + (size_t)kSplits * g.channels;   // one row for all samples: summed below
+    if (dshift && g.shift_sample == 0) per_sample = part + (size_t)2 * kSplits * g.channels;   // one row for all samples: summed below
     hipLaunchKernelGGL((gn_grad_apply_kernel<T, V, SWISH>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)dy, (const T *)x, mean,
                        rstd, (const float *)ws, (T *)dx, per_sample ? per_sample : dshift);
-    if (dbeta) column_sums(ws, rows, g.channels, part, dbeta, s);
-    if (dgamma) column_sums(ws + plane, rows, g.channels, part, dgamma, s);
-    if (per_sample) column_sums(per_sample, g.batch, g.channels, part, dshift, s);
+    if (dbeta || dgamma) column_sums(ws, rows, g.channels, part, dbeta, dgamma, 2, s);
+    if (per_sample) column_sums(per_sample, g.batch, g.channels, part, dshift, nullptr, 1, s);
     return check_launch("group norm backward: launch failed");
 }
 
@@ -552,9 +1147,20 @@ int idm_group_norm_forward(int device, const idm_group_norm_desc *d, const void 
     int rc = check_desc(d, false);
     if (rc != IDM_OK) return rc;
     if (d->batch == 0 || d->pixels == 0) return IDM_OK;
-    if (!x_dev || !y_dev || !mean_dev || !rstd_dev || !workspace_dev) return idm_set_error(IDM_ERR_INVALID, "group norm: null argument");
-    if (workspace_bytes < workspace_floats(*d, false) * sizeof(float)) return idm_set_error(IDM_ERR_INVALID, "group norm: workspace too small");
+    const size_t need = workspace_floats(*d, false) * sizeof(float);
+    if (!x_dev || !y_dev || !mean_dev || !rstd_dev || (need && !workspace_dev)) return idm_set_error(IDM_ERR_INVALID, "group norm: null argument");
+    if (workspace_bytes < need) return idm_set_error(IDM_ERR_INVALID, "group norm: workspace too small");
+    const bool aligned = aligned16({x_dev, y_dev, gamma_dev, beta_dev, shift_dev});
+    if (d->aligned && !aligned) return idm_set_error(IDM_ERR_INVALID, "group norm: a pointer is not aligned to 16 bytes as the descriptor says");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "group norm: no such device");
+    UnitPlan u;
+    if (plan_unit(*d, false, aligned, u)) {
+        UnitArgs a = unit_args(*d, u);
+        a.gamma = gamma_dev; a.beta = beta_dev; a.shift = shift_dev;
+        return by_piece(d->dtype, u.pieces, [&](auto t, auto p) {
+            return unit_forward<decltype(t), decltype(p)::value>(u, a, x_dev, y_dev, mean_dev, rstd_dev, (hipStream_t)stream);
+        });
+    }
     const int v = vec_of(*d, false, {x_dev, y_dev});
     Geometry g = geometry_of(*d, v);
     g.gamma = gamma_dev; g.beta = beta_dev; g.shift = shift_dev;
@@ -575,7 +1181,19 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
         return idm_set_error(IDM_ERR_INVALID, "group norm backward: null argument");
     if (workspace_bytes < workspace_floats(*d, true) * sizeof(float))
         return idm_set_error(IDM_ERR_INVALID, "group norm backward: workspace too small");
+    const bool aligned = aligned16({dy_dev, x_dev, dx_dev, gamma_dev, beta_dev, shift_dev});
+    if (d->aligned && !aligned)
+        return idm_set_error(IDM_ERR_INVALID, "group norm backward: a pointer is not aligned to 16 bytes as the descriptor says");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "group norm backward: no such device");
+    UnitPlan u;
+    if (plan_unit(*d, true, aligned, u)) {
+        UnitArgs a = unit_args(*d, u);
+        a.gamma = gamma_dev; a.beta = beta_dev; a.shift = shift_dev;
+        return by_piece(d->dtype, u.pieces, [&](auto t, auto p) {
+            return unit_backward<decltype(t), decltype(p)::value>(u, a, dy_dev, x_dev, mean_dev, rstd_dev, dx_dev, dgamma_dev, dbeta_dev,
+                                                                  dshift_dev, (float *)workspace_dev, (hipStream_t)stream);
+        });
+    }
     const int v = vec_of(*d, true, {dy_dev, x_dev, dx_dev});
     Geometry g = geometry_of(*d, v);
     g.gamma = gamma_dev; g.beta = beta_dev; g.shift = shift_dev;

@@ -77,7 +77,7 @@ class GroupNormDesc(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("batch", C.c_int64), ("pixels", C.c_int64),
                 ("channels", C.c_int32), ("groups", C.c_int32), ("x_sample", C.c_int64), ("x_pixel", C.c_int64),
                 ("dy_sample", C.c_int64), ("dy_pixel", C.c_int64), ("shift_sample", C.c_int64), ("eps", C.c_float),
-                ("reserved", C.c_int32)]
+                ("aligned", C.c_int32)]
 
 
 class AdamWCfg(C.Structure):
@@ -138,6 +138,16 @@ SIGNATURES = {
 }
 
 _lib = None
+_raw_stream = None
+
+
+def stream(index: int) -> int:
+    """The hipStream_t of the current stream of device ``index`` (2 us through the public object, 0.1 us by torch's own short cut)."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
 
 
 def load():

@@ -9,6 +9,7 @@ the channels of a group.  ``shift`` (B, C), (1, C) or (C,) is the block's time v
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -39,44 +40,65 @@ def _layout(x):
     return x, x.numel() // max(1, shape[0]), c
 
 
-def _check(x, gamma, beta, shift, groups, activation):
+def _refuse(x, gamma, beta, shift, groups, activation):
+    """The reason why these arguments are refused; called once a check has failed, or for a shape that is new."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
-        raise ValueError("x must be a tensor (B, ..., C)")
+        return "x must be a tensor (B, ..., C)"
     if x.dtype not in DTYPES:
-        raise ValueError("x must be float32, bfloat16 or float16")
+        return "x must be float32, bfloat16 or float16"
     if activation not in ACTIVATIONS:
-        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+        return f"activation must be one of {tuple(ACTIVATIONS)}"
     b, c = x.shape[0], x.shape[-1]
     if not isinstance(groups, int) or groups <= 0 or c == 0 or c % groups:
-        raise ValueError(f"groups must divide the {c} channels")
+        return f"groups must divide the {c} channels"
     for name, t in (("gamma", gamma), ("beta", beta)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (c,) or t.device != x.device):
-            raise ValueError(f"{name} must be ({c},) float32 on the device of x")
+            return f"{name} must be ({c},) float32 on the device of x"
     if shift is not None and (shift.dtype != torch.float32 or shift.device != x.device or shift.shape not in ((b, c), (1, c), (c,))):
-        raise ValueError(f"shift must be ({b}, {c}), (1, {c}) or ({c},) float32 on the device of x")
+        return f"shift must be ({b}, {c}), (1, {c}) or ({c},) float32 on the device of x"
     if not x.is_cuda:
-        raise ValueError("x must be a CUDA tensor")
+        return "x must be a CUDA tensor"
+    return None
+
+
+def _check(x, gamma, beta, shift, groups, activation):
+    why = _refuse(x, gamma, beta, shift, groups, activation)
+    if why:
+        raise ValueError(why)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _aligned(pointers):
+    return int(not any(p & 15 for p in pointers if p))
+
+
 def _dense(t):
-    return None if t is None else t.contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _desc(x, groups, activation, sample, pixel, shift, eps=0.0, dy_sample=0, dy_pixel=0):
-    b, c = x.shape[0], x.shape[-1]
-    per_sample = shift is not None and shift.dim() == 2 and shift.shape[0] == b and b > 1
-    return _lib.GroupNormDesc(DTYPES[x.dtype], ACTIVATIONS[activation], b, x.numel() // max(1, b * c), c, groups, sample, pixel,
-                              dy_sample, dy_pixel, c if per_sample else 0, eps, 0)
-
-
-def _workspace(desc, backward, device):
+@functools.lru_cache(maxsize=256)
+def _plan(shape, dtype, groups, activation, strides, per_sample, eps, aligned, backward):
+    """(descriptor, bytes of workspace) of a call: a function of sizes alone."""
+    b, c = shape[0], shape[-1]
+    desc = _lib.GroupNormDesc(DTYPES[dtype], ACTIVATIONS[activation], b, shape.numel() // (b * c), c, groups, *strides,
+                              c if per_sample else 0, eps, aligned)
     size = C.c_size_t()
     _lib.check(_lib.load().idm_group_norm_workspace(C.byref(desc), backward, C.byref(size)))
-    return torch.empty(max(16, size.value), dtype=torch.uint8, device=device), size.value
+    return C.byref(desc), size.value, desc
+
+
+def _call(entry, x, plan, args):
+    dev = x.device
+    ws = torch.empty(max(16, plan[1]), dtype=torch.uint8, device=dev) if plan[1] else None
+    args = (dev.index, plan[0], *args, _ptr(ws), plan[1])
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(entry(*args, _lib.stream(dev.index)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(entry(*args, _lib.stream(dev.index)))
 
 
 def group_norm_forward(x, gamma, beta, groups: int = 8, *, shift=None, eps: float = 1e-3, activation: str = "swish"):
@@ -86,20 +108,19 @@ def group_norm_forward(x, gamma, beta, groups: int = 8, *, shift=None, eps: floa
     _check(x, gamma, beta, shift, groups, activation)
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
-    dev = x.device
     x, sample, pixel = _layout(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=dev)
+    shape = x.shape
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty((shape[0], groups), dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     if x.numel() == 0:
-        return y, stats[0].zero_(), stats[1].fill_(eps ** -0.5 if eps else math.inf)
+        return y, mean.zero_(), rstd.fill_(eps ** -0.5 if eps else math.inf)
     gamma, beta, shift = _dense(gamma), _dense(beta), _dense(shift)
-    desc = _desc(x, groups, activation, sample, pixel, shift, eps)
-    with torch.cuda.device(dev):
-        ws, size = _workspace(desc, 0, dev)
-        _lib.check(_lib.load().idm_group_norm_forward(dev.index, C.byref(desc), x.data_ptr(), _ptr(gamma), _ptr(beta), _ptr(shift),
-                                                      y.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(), ws.data_ptr(), size,
-                                                      torch.cuda.current_stream(dev).cuda_stream))
-    return y, stats[0], stats[1]
+    per_sample = shift is not None and shift.dim() == 2 and 1 < shape[0] == shift.shape[0]
+    at = _ptr(x), _ptr(gamma), _ptr(beta), _ptr(shift), _ptr(y)
+    plan = _plan(shape, x.dtype, groups, activation, (sample, pixel, 0, 0), per_sample, eps, _aligned(at), 0)
+    _call(_lib.load().idm_group_norm_forward, x, plan, (*at, mean.data_ptr(), rstd.data_ptr()))
+    return y, mean, rstd
 
 
 def group_norm_backward(dy, x, mean, rstd, gamma, beta, groups: int = 8, *, shift=None, activation: str = "swish"):
@@ -107,31 +128,29 @@ def group_norm_backward(dy, x, mean, rstd, gamma, beta, groups: int = 8, *, shif
     shift are, dshift has the shape of shift.  The arguments after ``dy`` are those of the forward call and its statistics.
     Equal inputs give equal bits."""
     _check(x, gamma, beta, shift, groups, activation)
-    b, c = x.shape[0], x.shape[-1]
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    shape = x.shape
+    if dy.shape != shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must have the shape, type and device of x")
     for t in (mean, rstd):
-        if t.shape != (b, groups) or t.dtype != torch.float32 or t.device != x.device:
-            raise ValueError(f"mean and rstd must be ({b}, {groups}) float32 on the device of x")
-    dev = x.device
+        if t.shape != (shape[0], groups) or t.dtype != torch.float32 or t.device != x.device:
+            raise ValueError(f"mean and rstd must be ({shape[0]}, {groups}) float32 on the device of x")
     x, sample, pixel = _layout(x)
     dy, dy_sample, dy_pixel = _layout(dy)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=torch.float32, device=dev)  # noqa: E731
+    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    new = lambda t: None if t is None else torch.empty(t.shape, dtype=torch.float32, device=x.device)  # noqa: E731
     dgamma, dbeta, dshift = new(gamma), new(beta), new(shift)
     if x.numel() == 0:
         for t in (dgamma, dbeta, dshift):
             if t is not None:
                 t.zero_()
         return dx, dgamma, dbeta, dshift
-    gamma, beta, shift, mean, rstd = (_dense(t) for t in (gamma, beta, shift, mean, rstd))
-    desc = _desc(x, groups, activation, sample, pixel, shift, 0.0, dy_sample, dy_pixel)
-    with torch.cuda.device(dev):
-        ws, size = _workspace(desc, 1, dev)
-        _lib.check(_lib.load().idm_group_norm_backward(dev.index, C.byref(desc), dy.data_ptr(), x.data_ptr(), mean.data_ptr(),
-                                                       rstd.data_ptr(), _ptr(gamma), _ptr(beta), _ptr(shift), dx.data_ptr(),
-                                                       _ptr(dgamma), _ptr(dbeta), _ptr(dshift), ws.data_ptr(), size,
-                                                       torch.cuda.current_stream(dev).cuda_stream))
+    gamma, beta, shift, mean, rstd = _dense(gamma), _dense(beta), _dense(shift), _dense(mean), _dense(rstd)
+    per_sample = shift is not None and shift.dim() == 2 and 1 < shape[0] == shift.shape[0]
+    at = _ptr(gamma), _ptr(beta), _ptr(shift), _ptr(dx)
+    aligned = _aligned((*at, dy.data_ptr(), x.data_ptr()))
+    plan = _plan(shape, x.dtype, groups, activation, (sample, pixel, dy_sample, dy_pixel), per_sample, 0.0, aligned, 1)
+    _call(_lib.load().idm_group_norm_backward, x, plan, (dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), *at, _ptr(dgamma),
+                                                         _ptr(dbeta), _ptr(dshift)))
     return dx, dgamma, dbeta, dshift
 
 

@@ -16,6 +16,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
+from array import array
+from itertools import repeat
 
 import torch
 
@@ -49,59 +52,79 @@ def adamw_state(params, moment_bits: int = 32) -> dict:
 def _check_state(state, total, dev):
     """Moment bits of a state that fits `total` entries (None: any whole number of blocks) on `dev`."""
     eight = state["m"].dtype == torch.uint8
-    kinds = {"step": torch.int64, "m": torch.uint8 if eight else torch.float32, "v": torch.uint8 if eight else torch.float32}
-    if eight:
-        kinds.update(m_base=torch.int16, v_base=torch.int16)
+    kind = torch.uint8 if eight else torch.float32
     total = state["m"].numel() if total is None else total
-    for k, kind in kinds.items():
-        t, n = state[k], 1 if k == "step" else total // BLOCK if k.endswith("base") else total
-        if t.dtype != kind or t.numel() != n or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"state[{k!r}] must be {n} dense {kind} values on {dev}: make it with adamw_state for these parameters")
+    for k in ("step", "m", "v", "m_base", "v_base") if eight else ("step", "m", "v"):
+        t = state[k]
+        want, n = (torch.int64, 1) if k == "step" else (torch.int16, total // BLOCK) if k.endswith("base") else (kind, total)
+        if t.dtype != want or t.numel() != n or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"state[{k!r}] must be {n} dense {want} values on {dev}: make it with adamw_state for these parameters")
     return 8 if eight else 32
 
 
-def _pointers(ts):
-    return (C.c_void_p * len(ts))(*[None if t is None else t.data_ptr() for t in ts])
+def _call(entry, dev, args):
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(entry(dev.index, *args, _lib.stream(dev.index)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(entry(dev.index, *args, _lib.stream(dev.index)))
 
 
 def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01):
     """One step, in place: ``params``, and ``state`` of :func:`adamw_state`.  ``weight_decay`` is a number, or one per tensor.  A
     gradient that is None leaves its tensor and moments as they are.  Enqueued on the current stream; a captured step replays with
     the tensors, lr and decays that it was captured with, while its step count goes on."""
+    # (loops over the tensors are map() of tensor methods: at 66 tensors the host is slower than the device)
     params, grads = list(params), list(grads)
-    if not params or len(params) != len(grads):
+    n = len(params)
+    if not n or n != len(grads):
         raise ValueError("params and grads must be lists of the same length, not empty")
+    given, with_grad = grads, params
+    if any(map(operator.is_, grads, repeat(None))):
+        with_grad = [p for p, g in zip(params, grads) if g is not None]
+        given = [g for g in grads if g is not None]
+    Tensor = torch.Tensor
     dev, ptype = params[0].device, params[0].dtype
-    gtype = next((g.dtype for g in grads if g is not None), ptype)
+    gtype = given[0].dtype if given else ptype
     if ptype not in DTYPES or gtype not in DTYPES:
         raise ValueError("parameters and gradients must be float32, bfloat16 or float16")
-    sizes = [p.numel() for p in params]
-    for p, g in zip(params, grads):
-        if p.dtype != ptype or p.device != dev or not p.is_contiguous():
-            raise ValueError("parameters must be dense, of one type and on one device")
-        if g is not None and (g.dtype != gtype or g.device != dev or g.shape != p.shape):
-            raise ValueError("a gradient must have its parameter's shape and device, and all gradients one type")
-    grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
-    n = len(params)
-    decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
-    if len(decay) != n:
+    where = set(map(Tensor.get_device, params)) | set(map(Tensor.get_device, given))
+    if {p.dtype for p in params} != {ptype} or len(where) != 1 or not all(map(Tensor.is_contiguous, params)):
+        raise ValueError("parameters must be dense, of one type and on one device")
+    if given and ({g.dtype for g in given} != {gtype} or list(map(Tensor.size, given)) != list(map(Tensor.size, with_grad))):
+        raise ValueError("a gradient must have its parameter's shape and device, and all gradients one type")
+    if not all(map(Tensor.is_contiguous, given)):
+        given = [g.contiguous() for g in given]
+    sizes = array("q", map(Tensor.numel, params))
+    if isinstance(weight_decay, (int, float)):
+        lowest, decay = weight_decay, array("f", (weight_decay,)) * n
+    else:
+        decay = array("f", weight_decay)
+        lowest = min(decay) if len(decay) == n else None
+    if lowest is None:
         raise ValueError("weight_decay must be a number or one per tensor")
-    if not (math.isfinite(lr) and lr >= 0 and math.isfinite(eps) and eps >= 0 and all(0 <= b < 1 for b in betas)
-            and all(math.isfinite(w) and w >= 0 for w in decay)):
+    if not (math.isfinite(lr) and lr >= 0 and math.isfinite(eps) and eps >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1
+            and lowest >= 0 and all(map(math.isfinite, decay))):
         raise ValueError("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)")
-    bits = _check_state(state, sum(_room(s) for s in sizes), dev)
+    bits = _check_state(state, sum(-(-s // BLOCK) for s in sizes) * BLOCK, dev)
     if dev.type != "cuda":
         raise ValueError("parameters must be CUDA tensors")
+    at = array("q", map(Tensor.data_ptr, params))
+    if given is grads or len(given) == n:
+        grad_at = array("q", map(Tensor.data_ptr, given))
+    else:
+        it = iter(given)
+        grad_at = array("q", [0 if g is None else next(it).data_ptr() for g in grads])
     cfg = _lib.AdamWCfg(DTYPES[ptype], DTYPES[gtype], bits, 0, lr, betas[0], betas[1], eps)
-    base = [state[k].data_ptr() if bits == 8 else None for k in ("m_base", "v_base")]
-    with torch.cuda.device(dev):
-        scratch = torch.empty(16, dtype=torch.uint8, device=dev)
-        _lib.check(_lib.load().idm_adamw_step(dev.index, C.byref(cfg), n, _pointers(params), _pointers(grads), (C.c_int64 * n)(*sizes),
-                                              (C.c_float * n)(*decay), state["m"].data_ptr(), state["v"].data_ptr(), *base,
-                                              state["m"].numel(), state["step"].data_ptr(), scratch.data_ptr(),
-                                              torch.cuda.current_stream(dev).cuda_stream))
+    base = (state["m_base"].data_ptr(), state["v_base"].data_ptr()) if bits == 8 else (None, None)
+    scratch = torch.empty(2, dtype=torch.int64, device=dev)
+    _call(_lib.load().idm_adamw_step, dev, (C.byref(cfg), n, at.buffer_info()[0], grad_at.buffer_info()[0], sizes.buffer_info()[0],
+                                            decay.buffer_info()[0], state["m"].data_ptr(), state["v"].data_ptr(), *base,
+                                            state["m"].numel(), state["step"].data_ptr(), scratch.data_ptr()))
     # the kernel writes behind autograd's back: a backward pass that saved a parameter has to see that it changed
-    torch.autograd.graph.increment_version([p for p in params if p.requires_grad])
+    leaves = [p for p in params if p.requires_grad]
+    if leaves:
+        torch.autograd.graph.increment_version(leaves)
 
 
 def adamw_moments(state):
@@ -114,10 +137,9 @@ def adamw_moments(state):
     if dev.type != "cuda":
         raise ValueError("the state must be on a CUDA device")
     n = state["m"].numel()
-    m, v = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().idm_adamw_moments(dev.index, *(state[k].data_ptr() for k in ("m", "v", "m_base", "v_base")),
-                                                 m.data_ptr(), v.data_ptr(), n, torch.cuda.current_stream(dev).cuda_stream))
+    m = torch.empty(n, dtype=torch.float32, device=dev)
+    v = torch.empty_like(m)
+    _call(_lib.load().idm_adamw_moments, dev, (*(state[k].data_ptr() for k in ("m", "v", "m_base", "v_base")), m.data_ptr(), v.data_ptr(), n))
     return m, v
 
 

@@ -363,10 +363,11 @@ typedef struct {
     int64_t x_sample, x_pixel, dy_sample, dy_pixel;
     int64_t shift_sample;   /* stride of a sample in shift: channels, or 0 when all samples share one row */
     float eps;              /* forward only */
-    int32_t reserved;
+    int32_t aligned;        /* 1: x, y, dy, dx, gamma, beta and shift of the call are multiples of 16 bytes (checked); less workspace */
 } idm_group_norm_desc;
 
-/* Bytes of workspace that the forward (backward = 0) or backward call of this shape needs at most.  Launches nothing. */
+/* Bytes of workspace that the forward (backward = 0) or backward call of this shape needs at most; 0: the pointer may be NULL.
+ * Launches nothing. */
 int idm_group_norm_workspace(const idm_group_norm_desc *d, int backward, size_t *bytes);
 
 /* u = x + shift[b, c];  xhat = (u - mean) * rstd with mean and rstd = 1 / sqrt(var + eps) over the pixels and channels of a

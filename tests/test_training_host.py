@@ -31,7 +31,7 @@ def test_norm_refuses():
 
 def norm_desc(**over):
     f = dict(dtype=0, activation=1, batch=2, pixels=16, channels=16, groups=8, x_sample=256, x_pixel=16, dy_sample=256, dy_pixel=16,
-             shift_sample=0, eps=1e-3, reserved=0)
+             shift_sample=0, eps=1e-3, aligned=0)
     f.update(over)
     return _lib.GroupNormDesc(**f)
 
@@ -60,6 +60,12 @@ def test_norm_entry_points_refuse():
     assert lib.idm_group_norm_forward(0, C.byref(d), *[16] * 8, 8, None) == -1 and b"workspace" in lib.idm_last_error()
     assert lib.idm_group_norm_backward(0, C.byref(d), *[16] * 12, 8, None) == -1 and b"workspace" in lib.idm_last_error()
     assert lib.idm_group_norm_forward(0, None, *[16] * 8, 1 << 30, None) == -1
+    d = norm_desc(aligned=1)
+    assert lib.idm_group_norm_workspace(C.byref(d), 0, C.byref(size)) == 0 and size.value == 0
+    for k in (0, 1, 2, 3, 4):      # x, gamma, beta, shift, y
+        args = [16] * 8
+        args[k] = 24
+        assert lib.idm_group_norm_forward(0, C.byref(d), *args, 1 << 30, None) == -1 and b"aligned" in lib.idm_last_error()
 
 
 def test_layout_of_strided_maps():
