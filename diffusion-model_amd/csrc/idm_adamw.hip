@@ -25,16 +25,17 @@
 
 namespace {
 
-constexpr int BLOCK = IDM_ADAMW_BLOCK;      // entries that share a window = 4 per lane of one wavefront
+constexpr int BLOCK = IDM_ADAMW_BLOCK;      // entries that share a window
 constexpr int CHUNK = 4096;                 // entries of one workgroup
-constexpr int TENSORS = 64;                 // tensors of one launch (their table travels in the kernel arguments)
+constexpr int TENSORS = 96;                 // tensors of one launch (their table travels in the kernel arguments, at most 4 KB)
 constexpr uint32_t ROT_A = 0xC13FA9A9u, ROT_B = 0x91E10DA5u;
 
 struct Table {
     void *p[TENSORS];
     const void *g[TENSORS];
-    int64_t n[TENSORS], at[TENSORS];        // entries; index of the first one in the moments
-    int64_t first[TENSORS + 1];             // first chunk
+    int64_t n[TENSORS];                     // entries
+    uint32_t at[TENSORS];                   // block of the first one in the moments
+    int32_t first[TENSORS + 1];             // first chunk
     float keep[TENSORS];                    // 1 - lr wd
     int count;
 };
@@ -53,14 +54,6 @@ __global__ void adamw_begin_kernel(int64_t *step, double lr, double b1, double b
     c->t = (uint32_t)t;
 }
 
-// The float32 bits of |x|, rounded to a multiple of 2^20 by the dither: eighths of a binade.  Not finite: 2047.
-DEVI int place(uint32_t bits, uint32_t turn)
-{
-    const uint32_t size = bits & 0x7fffffffu;
-    const uint32_t q = (size + (turn >> 12)) >> 20;
-    return size < 0x7f800000u ? (int)(q < 2039u ? q : 2039u) : 2047;
-}
-
 DEVI float value_m(uint32_t code, int base)
 {
     const uint32_t c = code & 127u;
@@ -68,14 +61,50 @@ DEVI float value_m(uint32_t code, int base)
 }
 DEVI float value_v(uint32_t code, int base) { return __uint_as_float(code ? (code + (uint32_t)base) << 20 : 0u); }
 
-DEVI int wave_max(int x)
+// The float32 bits of |x|, rounded to a multiple of 2^20 by the dither: eighths of a binade
+DEVI uint32_t place(uint32_t size, uint32_t turn) { return (size + (turn >> 12)) >> 20; }
+// The same where x may not be finite (2047), or may round up to what infinity has
+DEVI uint32_t place_any(uint32_t size, uint32_t turn)
 {
+    const uint32_t q = place(size, turn);
+    return size >= 0x7f800000u ? 2047u : q < 2039u ? q : 2039u;
+}
+
+// N entries of a thread.  `full`: all are there and the address is aligned; else one by one, those below n only.
+template <typename T, int N> DEVI void load_entries(const T *p, int64_t i, int64_t n, bool full, float out[N])
+{
+    typedef __attribute__((ext_vector_type(N))) T vec;
+    if (full) {
+        const vec v = *(const vec *)(p + i);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const int o = __shfl_xor(x, off, 64);
-        x = o > x ? o : x;
+        for (int j = 0; j < N; ++j) out[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = i + j < n ? (float)p[i + j] : 0.0f;
     }
-    return x;
+}
+template <typename T, int N> DEVI void store_entries(T *p, int64_t i, int64_t n, bool full, const float in[N])
+{
+    typedef __attribute__((ext_vector_type(N))) T vec;
+    if (full) {
+        vec v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (T)in[j];
+        *(vec *)(p + i) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (i + j < n) p[i + j] = (T)in[j];
+    }
+}
+
+// sqrt and 1 / x by the instructions (one unit in the last place each; the moments do not depend on them).  v_sqrt_f32 takes
+// denormals for zero, hence the scale.
+DEVI float root_of(float v)
+{
+    const bool small = v < 0x1p-90f;
+    const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v);
+    return small ? r * 0x1p-32f : r;
 }
 
 template <typename PT, typename GT, bool EIGHT>
@@ -83,7 +112,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
                                                     float eps, void *__restrict__ m_all, void *__restrict__ v_all,
                                                     int16_t *__restrict__ m_base, int16_t *__restrict__ v_base)
 {
-    const int64_t chunk = blockIdx.x;
+    constexpr int N = EIGHT ? 8 : 4;           // entries of a thread: 16-byte loads of 16-bit parameters beside 8-byte ones of codes
+    constexpr int LANES = BLOCK / N;           // that share a window
+    const int chunk = blockIdx.x;
     int k = 0, hi = tab.count;   // the tensor whose chunks hold this one
     while (hi - k > 1) {
         const int mid = (k + hi) >> 1;
@@ -91,66 +122,76 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
     }
     PT *p = (PT *)tab.p[k];
     const GT *g = (const GT *)tab.g[k];
-    const int64_t n = tab.n[k], at = tab.at[k], i0 = (chunk - tab.first[k]) * CHUNK;
+    const int64_t n = tab.n[k], at = (int64_t)tab.at[k] * BLOCK, i0 = (int64_t)(chunk - tab.first[k]) * CHUNK;
+    const bool aligned = ((uintptr_t)p % (N * sizeof(PT)) | (uintptr_t)g % (N * sizeof(GT))) == 0;
     const float keep = tab.keep[k], size = coef->size, root = coef->root;
     const uint32_t t = coef->t;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int blk = wave; blk < CHUNK / BLOCK; blk += 4) {
-        const int64_t i = i0 + blk * BLOCK + lane * 4;
-        if (i0 + blk * BLOCK >= n) break;          // (the same for the whole wavefront)
-        float pv[4], gv[4], m[4], v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool in = i + j < n;
-            pv[j] = in ? (float)p[i + j] : 0.0f;
-            gv[j] = in ? (float)g[i + j] : 0.0f;
-        }
-        const int64_t w = (at + i0) / BLOCK + blk;   // the block among the moments
+#pragma unroll 2
+    for (int64_t i = i0 + threadIdx.x * N; i < i0 + CHUNK; i += 256 * N) {
+        if (i / BLOCK * BLOCK >= n) break;     // (the same for all lanes of a block)
+        const bool full = aligned && i + N <= n;
+        float pv[N], gv[N], m[N], v[N];
+        load_entries<PT, N>(p, i, n, full, pv);
+        load_entries<GT, N>(g, i, n, full, gv);
+        const int64_t w = (at + i) / BLOCK;    // the block among the moments
         if constexpr (EIGHT) {
-            const uint32_t cm = *(const uint32_t *)((const uint8_t *)m_all + at + i), cv = *(const uint32_t *)((const uint8_t *)v_all + at + i);
+            const uint2 cm = *(const uint2 *)((const uint8_t *)m_all + at + i), cv = *(const uint2 *)((const uint8_t *)v_all + at + i);
             const int bm = m_base[w], bv = v_base[w];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m[j] = value_m(cm >> 8 * j & 255u, bm);
-                v[j] = value_v(cv >> 8 * j & 255u, bv);
+            for (int j = 0; j < N; ++j) {
+                m[j] = value_m((j < 4 ? cm.x : cm.y) >> 8 * (j & 3) & 255u, bm);
+                v[j] = value_v((j < 4 ? cv.x : cv.y) >> 8 * (j & 3) & 255u, bv);
             }
         } else {
             const f32x4 mm = *(const f32x4 *)((const float *)m_all + at + i), vv = *(const f32x4 *)((const float *)v_all + at + i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { m[j] = mm[j]; v[j] = vv[j]; }
+            for (int j = 0; j < N; ++j) { m[j] = mm[j]; v[j] = vv[j]; }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < N; ++j) {
             m[j] = m[j] * b1 + gv[j] * c1;
             v[j] = v[j] * b2 + (gv[j] * gv[j]) * c2;
-            pv[j] = pv[j] * keep - size * (m[j] / (sqrtf(v[j]) * root + eps));
-            if (i + j < n) p[i + j] = (PT)pv[j];
+            pv[j] = pv[j] * keep - size * (m[j] * __builtin_amdgcn_rcpf(root_of(v[j]) * root + eps));
         }
+        store_entries<PT, N>(p, i, n, full, pv);
         if constexpr (EIGHT) {
-            int qm[4], qv[4], tm = 0, tv = 0;
+            typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+            uint32_t qm[N], qv[N], top = 0, tm = 0, tv = 0;
+            const uint32_t id = (uint32_t)(at + i), ta = id * ROT_A + t * ROT_B, tb = id * ROT_B + t * ROT_A;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t id = (uint32_t)(at + i + j);
-                qm[j] = place(__float_as_uint(m[j]), id * ROT_A + t * ROT_B);
-                qv[j] = place(__float_as_uint(v[j]), id * ROT_B + t * ROT_A);
-                tm = qm[j] < 2047 && qm[j] > tm ? qm[j] : tm;
-                tv = qv[j] < 2047 && qv[j] > tv ? qv[j] : tv;
+            for (int j = 0; j < N; ++j) {
+                const uint32_t sm = __float_as_uint(m[j]) & 0x7fffffffu, sv = __float_as_uint(v[j]) & 0x7fffffffu;
+                qm[j] = place(sm, ta + j * ROT_A);
+                qv[j] = place(sv, tb + j * ROT_B);
+                tm = qm[j] > tm ? qm[j] : tm;
+                tv = qv[j] > tv ? qv[j] : tv;
             }
-            tm = wave_max(tm);
-            tv = wave_max(tv);
-            const int bm = tm > 127 ? tm - 127 : 0, bv = tv > 255 ? tv - 255 : 0;
-            uint32_t cm = 0, cv = 0;
+            if ((tm > tv ? tm : tv) >= 2039u) {   // rare: near the largest float32 or not finite
+                tm = tv = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                int a = qm[j] - bm, b = qv[j] - bv;
-                a = a < 0 ? 0 : a > 127 ? 127 : a;
-                b = qv[j] == 0 ? 0 : b < 1 ? 1 : b > 255 ? 255 : b;
-                cm |= ((uint32_t)a | __float_as_uint(m[j]) >> 31 << 7) << 8 * j;
-                cv |= (uint32_t)b << 8 * j;
+                for (int j = 0; j < N; ++j) {
+                    qm[j] = place_any(__float_as_uint(m[j]) & 0x7fffffffu, ta + j * ROT_A);
+                    qv[j] = place_any(__float_as_uint(v[j]) & 0x7fffffffu, tb + j * ROT_B);
+                    if (qm[j] < 2047u) tm = qm[j] > tm ? qm[j] : tm;
+                    if (qv[j] < 2047u) tv = qv[j] > tv ? qv[j] : tv;
+                }
             }
-            *(uint32_t *)((uint8_t *)m_all + at + i) = cm;
-            *(uint32_t *)((uint8_t *)v_all + at + i) = cv;
-            if (lane == 0) {
+            top = tm | tv << 16;                  // both maxima in one exchange
+#pragma unroll
+            for (int off = LANES / 2; off >= 1; off >>= 1)
+                top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                             __builtin_bit_cast(u16x2, (uint32_t)__shfl_xor((int)top, off, 64))));
+            const int bm = max((int)(top & 0xffffu) - 127, 0), bv = max((int)(top >> 16) - 255, 0);
+            uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int a = min(max((int)qm[j] - bm, 0), 127), b = min(max((int)qv[j] - bv, min((int)qv[j], 1)), 255);
+                cm[j >> 2] |= ((uint32_t)a | (__float_as_uint(m[j]) >> 24 & 128u)) << 8 * (j & 3);
+                cv[j >> 2] |= (uint32_t)b << 8 * (j & 3);
+            }
+            *(uint2 *)((uint8_t *)m_all + at + i) = uint2{cm[0], cm[1]};
+            *(uint2 *)((uint8_t *)v_all + at + i) = uint2{cv[0], cv[1]};
+            if ((threadIdx.x & (LANES - 1)) == 0) {
                 m_base[w] = (int16_t)bm;
                 v_base[w] = (int16_t)bv;
             }
@@ -227,6 +268,7 @@ try {
         if ((uintptr_t)params_dev[i] % pb || (uintptr_t)grads_dev[i] % gb) return idm_set_error(IDM_ERR_INVALID, "adamw: misaligned tensor");
         spans.push_back({(uintptr_t)params_dev[i], (uintptr_t)params_dev[i] + (size_t)sizes[i] * pb});
     }
+    if (total / BLOCK > 0xffffffff) return idm_set_error(IDM_ERR_INVALID, "adamw: more than 2^40 entries");
     if (total != moments) return idm_set_error(IDM_ERR_INVALID, "adamw: the moments were made for other tensors (each takes its size rounded up to 256 entries)");
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
@@ -244,7 +286,7 @@ try {
     tab.count = 0;
     auto flush = [&]() -> int {
         if (!tab.count) return IDM_OK;
-        tab.first[tab.count] = chunks;
+        tab.first[tab.count] = (int32_t)chunks;
         auto go = [&](auto p, auto g) {
             using PT = decltype(p);
             using GT = decltype(g);
@@ -261,7 +303,7 @@ try {
     for (int64_t i = 0; i < n_tensors; at += room_of(sizes[i]), ++i) {
         if (!sizes[i] || !grads_dev[i]) continue;      // no gradient: the tensor and its moments stay as they are
         // a tensor of more chunks than one launch has workgroups is cut
-        const int64_t most = (int64_t)1 << 30;
+        const int64_t most = (int64_t)1 << 28;
         for (int64_t lo = 0; lo < sizes[i]; lo += most * CHUNK) {
             const int64_t n = std::min<int64_t>(sizes[i] - lo, most * CHUNK), c = (n + CHUNK - 1) / CHUNK;
             if (tab.count == TENSORS || chunks + c > 0x7fffffff) {
@@ -272,8 +314,8 @@ try {
             tab.p[k] = (char *)params_dev[i] + lo * pb;
             tab.g[k] = (const char *)grads_dev[i] + lo * gb;
             tab.n[k] = n;
-            tab.at[k] = at + lo;
-            tab.first[k] = chunks;
+            tab.at[k] = (uint32_t)((at + lo) / BLOCK);
+            tab.first[k] = (int32_t)chunks;
             tab.keep[k] = (float)(1.0 - cfg->lr * (double)weight_decay[i]);
             chunks += c;
         }
