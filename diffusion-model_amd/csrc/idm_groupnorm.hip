@@ -188,18 +188,25 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
 {
     __shared__ float s_mean[THREADS], s_rstd[THREADS];
     const Place w = place_of(g, blockIdx.x, THREADS * V);
-    const int np = g.nchunk * g.tpg, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int k = wave; k < w.ng; k += THREADS / 64) {
-        const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
+    // the partials of a group are joined by `lanes` lanes, all groups of the tile at once where there are few
+    const int np = g.nchunk * g.tpg;
+    int lanes = 64;
+    while (lanes > 8 && lanes * w.ng > THREADS) lanes >>= 1;
+    const int lane = threadIdx.x & (lanes - 1);
+    for (int k0 = 0; k0 < w.ng; k0 += THREADS / lanes) {
+        const int k = k0 + (int)threadIdx.x / lanes;
         Moments t = {0.0f, 0.0f, 0.0f};
-        for (int i = lane; i < np; i += 64) {
-            const float *o = pp + (int64_t)i * g.groups * 3;
-            t = join(t, {o[0], o[1], o[2]});
+        if (k < w.ng) {
+            const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
+#pragma unroll 4
+            for (int i = lane; i < np; i += lanes) {
+                const float *o = pp + (int64_t)i * g.groups * 3;
+                t = join(t, {o[0], o[1], o[2]});
+            }
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1)
+        for (int off = lanes >> 1; off >= 1; off >>= 1)
             t = join(t, {__shfl_xor(t.n, off, 64), __shfl_xor(t.mean, off, 64), __shfl_xor(t.m2, off, 64)});
-        if (lane) continue;
+        if (k >= w.ng || lane) continue;
         const float rstd = 1.0f / sqrtf(t.m2 / t.n + g.eps);
         s_mean[k] = t.mean;
         s_rstd[k] = rstd;
@@ -331,27 +338,35 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
 {
     __shared__ float s_a[THREADS], s_b[THREADS];
     const Place w = place_of(g, blockIdx.x, THREADS * V);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t plane = g.batch * g.nchunk * g.channels;
     const float *sb = sums + w.b * g.nchunk * g.channels;
     const float inv_n = 1.0f / ((float)g.pixels * (float)g.gc);
-    for (int k = wave; k < w.ng; k += THREADS / 64) {
-        const int gc0 = (w.g0 + k) * g.gc;
+    int lanes = 64;
+    while (lanes > 8 && lanes * w.ng > THREADS) lanes >>= 1;
+    const int lane = threadIdx.x & (lanes - 1);
+    for (int k0 = 0; k0 < w.ng; k0 += THREADS / lanes) {
+        const int k = k0 + (int)threadIdx.x / lanes, gc0 = (w.g0 + k) * g.gc;
         float a = 0.0f, b = 0.0f;
+        if (k < w.ng) {
+            // lanes run over the channels first; a lane's channels are c0, c0 + dc, ... (mod gc) of chunks i0, ...
+            int i = lane / g.gc, c = lane - i * g.gc;
+            const int di = lanes / g.gc, dc = lanes - di * g.gc;
 #pragma unroll 4
-        for (int64_t e = lane; e < (int64_t)g.nchunk * g.gc; e += 64) {
-            const int64_t i = e / g.gc, c = gc0 + (e - i * g.gc);
-            const float *o = sb + i * g.channels + c;
-            const float gm = g.gamma ? g.gamma[c] : 1.0f;
-            a = __builtin_fmaf(gm, o[0], a);
-            b = __builtin_fmaf(gm, o[plane], b);
+            while (i < g.nchunk) {
+                const float *o = sb + (int64_t)i * g.channels + gc0 + c;
+                const float gm = g.gamma ? g.gamma[gc0 + c] : 1.0f;
+                a = __builtin_fmaf(gm, o[0], a);
+                b = __builtin_fmaf(gm, o[plane], b);
+                i += di;
+                c += dc;
+                if (c >= g.gc) { c -= g.gc; ++i; }
+            }
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
+        for (int off = lanes >> 1; off >= 1; off >>= 1) {
             a += __shfl_xor(a, off, 64);
             b += __shfl_xor(b, off, 64);
         }
-        if (lane == 0) {
+        if (k < w.ng && lane == 0) {
             s_a[k] = a * inv_n;
             s_b[k] = b * inv_n;
         }
@@ -871,7 +886,7 @@ Geometry geometry_of(const idm_group_norm_desc &d, int v)
     }
     // enough workgroups to fill the chip, none with less than a few vectors per thread
     const int rows = std::max(1, THREADS / std::min(THREADS, g.gpt * qg));
-    const int64_t most = std::max<int64_t>(1, g.pixels / (8 * rows)), want = (2048 + g.batch * g.ntile - 1) / (g.batch * g.ntile);
+    const int64_t most = std::max<int64_t>(1, g.pixels / (4 * rows)), want = (2048 + g.batch * g.ntile - 1) / (g.batch * g.ntile);
     int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, want, 1024}));
     g.chunk = (g.pixels + n - 1) / n;
     g.nchunk = (int)((g.pixels + g.chunk - 1) / g.chunk);

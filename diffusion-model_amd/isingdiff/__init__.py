@@ -35,5 +35,7 @@ _LAZY = {
 def __getattr__(name):
     if name in _LAZY:
         import importlib
-        return getattr(importlib.import_module("." + _LAZY[name], __name__), name)
+        value = getattr(importlib.import_module("." + _LAZY[name], __name__), name)
+        globals()[name] = value     # (the next access does not come here: an import statement costs 5 us each time)
+        return value
     raise AttributeError(name)

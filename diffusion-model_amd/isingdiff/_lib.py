@@ -138,28 +138,32 @@ SIGNATURES = {
 }
 
 _lib = None
-_raw_stream = None
+_current_device = _raw_stream = _on_device = None      # of torch, bound by load()
 
 
-def stream(index: int) -> int:
-    """The hipStream_t of the current stream of device ``index`` (2 us through the public object, 0.1 us by torch's own short cut)."""
-    global _raw_stream
-    if _raw_stream is None:
-        import torch
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    return _raw_stream(index)
+def call(entry, dev, args):
+    """``entry(device, *args, stream)`` on torch's current stream of ``dev``, with ``dev`` as the current device."""
+    index = dev.index
+    if _current_device() == index:
+        check(entry(index, *args, _raw_stream(index)))
+    else:
+        with _on_device(index):
+            check(entry(index, *args, _raw_stream(index)))
 
 
 def load():
     """Load the shared library (once) and bind every exported symbol."""
-    global _lib
+    global _lib, _current_device, _raw_stream, _on_device
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise IdmError(f"{LIB_PATH} not found: build it with `make -C diffusion-model_amd/csrc` "
                            "(there is no CPU fallback)")
         # PyTorch bundles its own HIP runtime (same SONAME as /opt/rocm's).  Import it first so that
         # this library binds to the runtime that owns torch's device pointers and streams.
-        import torch  # noqa: F401
+        import torch
+        _current_device, _on_device = torch.cuda.current_device, torch.cuda.device
+        # the hipStream_t of a device's current stream; by torch's own short cut where it has one (0.1 us instead of 2)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
         lib = C.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)

@@ -68,11 +68,12 @@ def _check(x, gamma, beta, shift, groups, activation):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _aligned(pointers):
-    return int(not any(p & 15 for p in pointers if p))
+def _like(x):
+    """A dense tensor like x."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _dense(t):
@@ -90,15 +91,10 @@ def _plan(shape, dtype, groups, activation, strides, per_sample, eps, aligned, b
     return C.byref(desc), size.value, desc
 
 
-def _call(entry, x, plan, args):
-    dev = x.device
-    ws = torch.empty(max(16, plan[1]), dtype=torch.uint8, device=dev) if plan[1] else None
-    args = (dev.index, plan[0], *args, _ptr(ws), plan[1])
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(entry(*args, _lib.stream(dev.index)))
-    else:
-        with torch.cuda.device(dev):
-            _lib.check(entry(*args, _lib.stream(dev.index)))
+def _call(entry, dev, plan, args):
+    desc, size, _ = plan
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _lib.call(entry, dev, (desc, *args, _ptr(ws), size))
 
 
 def group_norm_forward(x, gamma, beta, groups: int = 8, *, shift=None, eps: float = 1e-3, activation: str = "swish"):
@@ -110,16 +106,17 @@ def group_norm_forward(x, gamma, beta, groups: int = 8, *, shift=None, eps: floa
         raise ValueError("eps must be finite and not negative")
     x, sample, pixel = _layout(x)
     shape = x.shape
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     mean = torch.empty((shape[0], groups), dtype=torch.float32, device=x.device)
     rstd = torch.empty_like(mean)
     if x.numel() == 0:
         return y, mean.zero_(), rstd.fill_(eps ** -0.5 if eps else math.inf)
     gamma, beta, shift = _dense(gamma), _dense(beta), _dense(shift)
     per_sample = shift is not None and shift.dim() == 2 and 1 < shape[0] == shift.shape[0]
-    at = _ptr(x), _ptr(gamma), _ptr(beta), _ptr(shift), _ptr(y)
-    plan = _plan(shape, x.dtype, groups, activation, (sample, pixel, 0, 0), per_sample, eps, _aligned(at), 0)
-    _call(_lib.load().idm_group_norm_forward, x, plan, (*at, mean.data_ptr(), rstd.data_ptr()))
+    px, pg, pb, ps, py = x.data_ptr(), _ptr(gamma), _ptr(beta), _ptr(shift), y.data_ptr()
+    aligned = not (px | pg | pb | ps | py) & 15
+    plan = _plan(shape, x.dtype, groups, activation, (sample, pixel, 0, 0), per_sample, eps, aligned, 0)
+    _call(_lib.load().idm_group_norm_forward, x.device, plan, (px, pg, pb, ps, py, mean.data_ptr(), rstd.data_ptr()))
     return y, mean, rstd
 
 
@@ -136,8 +133,8 @@ def group_norm_backward(dy, x, mean, rstd, gamma, beta, groups: int = 8, *, shif
             raise ValueError(f"mean and rstd must be ({shape[0]}, {groups}) float32 on the device of x")
     x, sample, pixel = _layout(x)
     dy, dy_sample, dy_pixel = _layout(dy)
-    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=torch.float32, device=x.device)  # noqa: E731
+    dx = _like(x)
+    new = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
     dgamma, dbeta, dshift = new(gamma), new(beta), new(shift)
     if x.numel() == 0:
         for t in (dgamma, dbeta, dshift):
@@ -146,11 +143,11 @@ def group_norm_backward(dy, x, mean, rstd, gamma, beta, groups: int = 8, *, shif
         return dx, dgamma, dbeta, dshift
     gamma, beta, shift, mean, rstd = _dense(gamma), _dense(beta), _dense(shift), _dense(mean), _dense(rstd)
     per_sample = shift is not None and shift.dim() == 2 and 1 < shape[0] == shift.shape[0]
-    at = _ptr(gamma), _ptr(beta), _ptr(shift), _ptr(dx)
-    aligned = _aligned((*at, dy.data_ptr(), x.data_ptr()))
+    pd, px, pg, pb, ps, po = dy.data_ptr(), x.data_ptr(), _ptr(gamma), _ptr(beta), _ptr(shift), dx.data_ptr()
+    aligned = not (pd | px | pg | pb | ps | po) & 15
     plan = _plan(shape, x.dtype, groups, activation, (sample, pixel, dy_sample, dy_pixel), per_sample, 0.0, aligned, 1)
-    _call(_lib.load().idm_group_norm_backward, x, plan, (dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), *at, _ptr(dgamma),
-                                                         _ptr(dbeta), _ptr(dshift)))
+    _call(_lib.load().idm_group_norm_backward, x.device, plan, (pd, px, mean.data_ptr(), rstd.data_ptr(), pg, pb, ps, po, _ptr(dgamma),
+                                                                _ptr(dbeta), _ptr(dshift)))
     return dx, dgamma, dbeta, dshift
 
 

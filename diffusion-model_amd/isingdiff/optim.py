@@ -26,6 +26,7 @@ from . import _lib
 from .norm import DTYPES
 
 BLOCK = _lib.ADAMW_BLOCK
+assert BLOCK == 1 << 8
 
 
 def _room(n: int) -> int:
@@ -62,14 +63,6 @@ def _check_state(state, total, dev):
     return 8 if eight else 32
 
 
-def _call(entry, dev, args):
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(entry(dev.index, *args, _lib.stream(dev.index)))
-    else:
-        with torch.cuda.device(dev):
-            _lib.check(entry(dev.index, *args, _lib.stream(dev.index)))
-
-
 def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01):
     """One step, in place: ``params``, and ``state`` of :func:`adamw_state`.  ``weight_decay`` is a number, or one per tensor.  A
     gradient that is None leaves its tensor and moments as they are.  Enqueued on the current stream; a captured step replays with
@@ -100,13 +93,13 @@ def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), ep
         lowest, decay = weight_decay, array("f", (weight_decay,)) * n
     else:
         decay = array("f", weight_decay)
-        lowest = min(decay) if len(decay) == n else None
-    if lowest is None:
-        raise ValueError("weight_decay must be a number or one per tensor")
+        if len(decay) != n:
+            raise ValueError("weight_decay must be a number or one per tensor")
+        lowest = min(decay)
     if not (math.isfinite(lr) and lr >= 0 and math.isfinite(eps) and eps >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1
-            and lowest >= 0 and all(map(math.isfinite, decay))):
+            and lowest >= 0 and math.isfinite(sum(decay))):
         raise ValueError("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)")
-    bits = _check_state(state, sum(-(-s // BLOCK) for s in sizes) * BLOCK, dev)
+    bits = _check_state(state, sum([s + BLOCK - 1 >> 8 for s in sizes]) * BLOCK, dev)
     if dev.type != "cuda":
         raise ValueError("parameters must be CUDA tensors")
     at = array("q", map(Tensor.data_ptr, params))
@@ -118,7 +111,7 @@ def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), ep
     cfg = _lib.AdamWCfg(DTYPES[ptype], DTYPES[gtype], bits, 0, lr, betas[0], betas[1], eps)
     base = (state["m_base"].data_ptr(), state["v_base"].data_ptr()) if bits == 8 else (None, None)
     scratch = torch.empty(2, dtype=torch.int64, device=dev)
-    _call(_lib.load().idm_adamw_step, dev, (C.byref(cfg), n, at.buffer_info()[0], grad_at.buffer_info()[0], sizes.buffer_info()[0],
+    _lib.call(_lib.load().idm_adamw_step, dev, (C.byref(cfg), n, at.buffer_info()[0], grad_at.buffer_info()[0], sizes.buffer_info()[0],
                                             decay.buffer_info()[0], state["m"].data_ptr(), state["v"].data_ptr(), *base,
                                             state["m"].numel(), state["step"].data_ptr(), scratch.data_ptr()))
     # the kernel writes behind autograd's back: a backward pass that saved a parameter has to see that it changed
@@ -139,7 +132,7 @@ def adamw_moments(state):
     n = state["m"].numel()
     m = torch.empty(n, dtype=torch.float32, device=dev)
     v = torch.empty_like(m)
-    _call(_lib.load().idm_adamw_moments, dev, (*(state[k].data_ptr() for k in ("m", "v", "m_base", "v_base")), m.data_ptr(), v.data_ptr(), n))
+    _lib.call(_lib.load().idm_adamw_moments, dev, (*(state[k].data_ptr() for k in ("m", "v", "m_base", "v_base")), m.data_ptr(), v.data_ptr(), n))
     return m, v
 
 
