@@ -90,13 +90,13 @@ struct Place {
     int chunk, tile, c0, width, g0, ng;   // tile's first channel, channels, first group, groups (1 where a group spans tiles)
 };
 
-DEVI Place place_of(const Geometry &g, int64_t block, int part_channels)
+// Grid: x chunks and tiles, y and z samples
+DEVI Place place_of(const Geometry &g, int part_channels)
 {
     Place w;
-    w.tile = (int)(block % g.ntile);
-    const int64_t r = block / g.ntile;
-    w.chunk = (int)(r % g.nchunk);
-    w.b = r / g.nchunk;
+    w.chunk = (int)blockIdx.x / g.ntile;
+    w.tile = (int)blockIdx.x - w.chunk * g.ntile;
+    w.b = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
     w.p0 = w.chunk * g.chunk;
     w.p1 = w.p0 + g.chunk < g.pixels ? w.p0 + g.chunk : g.pixels;
     if (g.tpg == 1) {
@@ -120,7 +120,8 @@ __global__ __launch_bounds__(THREADS) void gn_stats_kernel(Geometry g, const T *
 {
     constexpr int U = 4;   // vectors taken together: their mean first, then the squared distances from it
     __shared__ Moments sh[THREADS];
-    const Place w = place_of(g, blockIdx.x, THREADS * V);
+    const Place w = place_of(g, THREADS * V);
+    if (w.b >= g.batch) return;
     const int q = w.width / V, rows = THREADS / q, r = threadIdx.x / q, cq = threadIdx.x - r * q;
     Moments mine = {0.0f, 0.0f, 0.0f};
     if (r < rows) {
@@ -187,7 +188,8 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
                                                            float *__restrict__ rstd_out)
 {
     __shared__ float s_mean[THREADS], s_rstd[THREADS];
-    const Place w = place_of(g, blockIdx.x, THREADS * V);
+    const Place w = place_of(g, THREADS * V);
+    if (w.b >= g.batch) return;
     // the partials of a group are joined by `lanes` lanes, all groups of the tile at once where there are few
     const int np = g.nchunk * g.tpg;
     int lanes = 64;
@@ -244,6 +246,30 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
     }
 }
 
+// Column sums of one plane (rows, cols) for 16 columns: rows split, split + splits, ... by 256 threads
+DEVI void sum_columns(const float *in, int64_t rows, int cols, int col0, int split, int splits, float *out)
+{
+    __shared__ float sh[16][17];
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, col = col0 + lane;
+    const float *p = in + col;
+    float s = 0.0f;
+    if (col < cols)
+#pragma unroll 8
+        for (int64_t r = split + (int64_t)row * splits; r < rows; r += 16 * (int64_t)splits) s += p[r * cols];
+    sh[row][lane] = s;
+    __syncthreads();
+    if (row == 0 && col < cols) {
+        float t[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t[k] = sh[k][lane];
+#pragma unroll
+        for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; ++k) t[k] += t[k + w];
+        out[(int64_t)split * cols + col] = t[0];
+    }
+}
+
 // xhat and dz of V channels of a pixel
 template <int V, bool SWISH>
 DEVI void grad_z(const float u[V], const float dy[V], const float add[V], float rstd, const float gamma[V], const float beta[V],
@@ -286,10 +312,11 @@ template <typename F> DEVI void sum_rows(float *buf, int rows, int width, F &&do
 template <typename T, int V, bool SWISH>
 __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const T *__restrict__ dy, const T *__restrict__ x,
                                                                const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                                               float *__restrict__ sums, bool with_xhat)
+                                                               float *__restrict__ sums, float2 *__restrict__ groups, bool with_xhat)
 {
-    __shared__ float sh[THREADS * V];
-    const Place w = place_of(g, blockIdx.x, THREADS * V);
+    __shared__ float sh[THREADS * V], by_channel[2][THREADS * V];
+    const Place w = place_of(g, THREADS * V);
+    if (w.b >= g.batch) return;
     const int q = w.width / V, rows = THREADS / q, r = threadIdx.x / q, cq = threadIdx.x - r * q;
     float acc[3][V];
 #pragma unroll
@@ -326,49 +353,66 @@ __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const
 #pragma unroll
             for (int j = 0; j < V; ++j) sh[(r * q + cq) * V + j] = acc[i][j];
         __syncthreads();
-        sum_rows(sh, rows, w.width, [&](int c, float s) { sums[i * plane + row + w.c0 + c] = s; });
+        sum_rows(sh, rows, w.width, [&](int c, float s) {
+            sums[i * plane + row + w.c0 + c] = s;
+            if (i < 2) by_channel[i][c] = (g.gamma ? g.gamma[w.c0 + c] : 1.0f) * s;
+        });
+    }
+    // a group's share of this chunk: the next kernel reads these instead of every channel's
+    const int part = g.tpg == 1 ? 0 : w.tile % g.tpg, per = g.tpg == 1 ? g.gc : w.width;
+    for (int k = threadIdx.x; k < w.ng; k += THREADS) {
+        float2 t = {0.0f, 0.0f};
+        for (int c = k * per; c < (k + 1) * per; ++c) {
+            t.x += by_channel[0][c];
+            t.y += by_channel[1][c];
+        }
+        groups[((w.b * g.nchunk + w.chunk) * g.tpg + part) * g.groups + w.g0 + k] = t;
     }
 }
 
 template <typename T, int V, bool SWISH>
 __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, const T *__restrict__ dy, const T *__restrict__ x,
                                                                 const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                                                const float *__restrict__ sums, T *__restrict__ dx,
-                                                                float *__restrict__ dshift)
+                                                                const float *__restrict__ sums, const float2 *__restrict__ groups,
+                                                                T *__restrict__ dx, float *__restrict__ dshift, float *dbeta, float *dgamma)
 {
     __shared__ float s_a[THREADS], s_b[THREADS];
-    const Place w = place_of(g, blockIdx.x, THREADS * V);
+    if ((int)blockIdx.x >= g.nchunk * g.ntile) {   // blocks behind the chunks add up the weight gradients
+        if (blockIdx.y || blockIdx.z) return;
+        const int64_t rows = g.batch * g.nchunk;
+        const int at = ((int)blockIdx.x - g.nchunk * g.ntile) * 16, per = (g.channels + 15) / 16 * 16, plane = at >= per;
+        float *out = plane ? dgamma : dbeta;
+        if (out) sum_columns(sums + plane * rows * g.channels, rows, g.channels, at - plane * per, 0, 1, out);
+        return;
+    }
+    const Place w = place_of(g, THREADS * V);
+    if (w.b >= g.batch) return;
     const int64_t plane = g.batch * g.nchunk * g.channels;
     const float *sb = sums + w.b * g.nchunk * g.channels;
     const float inv_n = 1.0f / ((float)g.pixels * (float)g.gc);
+    const int np = g.nchunk * g.tpg;
     int lanes = 64;
     while (lanes > 8 && lanes * w.ng > THREADS) lanes >>= 1;
     const int lane = threadIdx.x & (lanes - 1);
     for (int k0 = 0; k0 < w.ng; k0 += THREADS / lanes) {
-        const int k = k0 + (int)threadIdx.x / lanes, gc0 = (w.g0 + k) * g.gc;
-        float a = 0.0f, b = 0.0f;
+        const int k = k0 + (int)threadIdx.x / lanes;
+        float2 t = {0.0f, 0.0f};
         if (k < w.ng) {
-            // lanes run over the channels first; a lane's channels are c0, c0 + dc, ... (mod gc) of chunks i0, ...
-            int i = lane / g.gc, c = lane - i * g.gc;
-            const int di = lanes / g.gc, dc = lanes - di * g.gc;
+            const float2 *pp = groups + w.b * np * g.groups + w.g0 + k;
 #pragma unroll 4
-            while (i < g.nchunk) {
-                const float *o = sb + (int64_t)i * g.channels + gc0 + c;
-                const float gm = g.gamma ? g.gamma[gc0 + c] : 1.0f;
-                a = __builtin_fmaf(gm, o[0], a);
-                b = __builtin_fmaf(gm, o[plane], b);
-                i += di;
-                c += dc;
-                if (c >= g.gc) { c -= g.gc; ++i; }
+            for (int i = lane; i < np; i += lanes) {
+                const float2 o = pp[(int64_t)i * g.groups];
+                t.x += o.x;
+                t.y += o.y;
             }
         }
         for (int off = lanes >> 1; off >= 1; off >>= 1) {
-            a += __shfl_xor(a, off, 64);
-            b += __shfl_xor(b, off, 64);
+            t.x += __shfl_xor(t.x, off, 64);
+            t.y += __shfl_xor(t.y, off, 64);
         }
         if (k < w.ng && lane == 0) {
-            s_a[k] = a * inv_n;
-            s_b[k] = b * inv_n;
+            s_a[k] = t.x * inv_n;
+            s_b[k] = t.y * inv_n;
         }
     }
     __syncthreads();
@@ -823,30 +867,12 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
         sum_rows(total[i], g.rows * g.pack, width, [&](int k, float t) { sums[((int64_t)i * walkers + walker) * g.channels + c0 + k] = t; });
 }
 
-// Column sums of planes (rows, cols): block (16 columns, plane, split) adds rows split, split + splits, ...
+// Grid: x 16 columns, y planes, z splits
 __global__ __launch_bounds__(256) void gn_columns_kernel(const float *__restrict__ in, int64_t rows, int cols, int splits, float *__restrict__ out0,
                                                          float *__restrict__ out1)
 {
-    __shared__ float sh[16][17];
-    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, col = blockIdx.x * 16 + lane;
-    const float *p = in + (int64_t)blockIdx.y * rows * cols + col;
     float *out = blockIdx.y ? out1 : out0;
-    float s = 0.0f;
-    if (col < cols)
-#pragma unroll 8
-        for (int64_t r = blockIdx.z + (int64_t)row * splits; r < rows; r += 16 * (int64_t)splits) s += p[r * cols];
-    sh[row][lane] = s;
-    __syncthreads();
-    if (row == 0 && col < cols && out) {
-        float t[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) t[k] = sh[k][lane];
-#pragma unroll
-        for (int w = 8; w >= 1; w >>= 1)
-#pragma unroll
-            for (int k = 0; k < w; ++k) t[k] += t[k + w];
-        out[(int64_t)blockIdx.z * cols + col] = t[0];
-    }
+    if (out) sum_columns(in + (int64_t)blockIdx.y * rows * cols, rows, cols, blockIdx.x * 16, blockIdx.z, splits, out);
 }
 
 constexpr int kSplits = 64;
@@ -978,7 +1004,7 @@ size_t workspace_floats(const idm_group_norm_desc &d, bool backward)
             if ((d.channels / d.groups) % v) continue;
             const Geometry g = geometry_of(d, v);
             const size_t rows = (size_t)g.batch * g.nchunk;
-            most = std::max(most, backward ? 3 * rows * g.channels : rows * g.tpg * g.groups * 3);
+            most = std::max(most, backward ? rows * (3 * g.channels + 2 * g.tpg * g.groups) : rows * g.tpg * g.groups * 3);
         }
     if (backward) most += (size_t)2 * kSplits * d.channels + (d.shift_sample == 0 ? (size_t)d.batch * d.channels : 0);
     return most;
@@ -1079,7 +1105,7 @@ int check_desc(const idm_group_norm_desc *d, bool backward)
         return idm_set_error(IDM_ERR_INVALID, "group norm: channels must be a positive multiple of groups, batch and pixels not negative");
     if (!(d->eps >= 0.0f) || std::isinf(d->eps)) return idm_set_error(IDM_ERR_INVALID, "group norm: eps must be finite and not negative");
     if (d->channels > (1 << 20) || d->pixels > ((int64_t)1 << 40) || d->batch > ((int64_t)1 << 31))
-        return idm_set_error(IDM_ERR_INVALID, "group norm: more than 2^20 channels, 2^40 pixels or 2^31 samples");
+        return idm_set_error(IDM_ERR_INVALID, "group norm: more than 2^20 channels, 2^40 pixels or 2^30 samples");
     if (d->x_pixel < d->channels || (backward && d->dy_pixel < d->channels))
         return idm_set_error(IDM_ERR_INVALID, "group norm: a pixel's stride is less than its channels");
     if (d->x_sample < 0 || d->shift_sample < 0 || (backward && d->dy_sample < 0))
@@ -1092,17 +1118,23 @@ int check_launch(const char *what)
     return hipGetLastError() == hipSuccess ? IDM_OK : idm_set_error(IDM_ERR_HIP, what);
 }
 
+// samples in y and z; `more` blocks behind the chunks and tiles
+dim3 chunk_grid(const Geometry &g, int more)
+{
+    const int64_t y = std::min<int64_t>(g.batch, 32768);
+    return dim3((unsigned)(g.nchunk * g.ntile + more), (unsigned)y, (unsigned)((g.batch + y - 1) / y));
+}
+
 template <typename T, int V>
 int forward_launch(const idm_group_norm_desc &d, const Geometry &g, const void *x, void *y, float *mean, float *rstd, float *ws,
                    hipStream_t s)
 {
-    const int64_t blocks = g.batch * g.nchunk * g.ntile;
-    if (blocks > 0x7fffffff) return idm_set_error(IDM_ERR_INVALID, "group norm: batch too large");
-    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)x, ws);
+    const dim3 blocks = chunk_grid(g, 0);
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), blocks, dim3(THREADS), 0, s, g, (const T *)x, ws);
     if (d.activation == IDM_ACT_SWISH)
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, true>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)x, ws, (T *)y, mean, rstd);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, true>), blocks, dim3(THREADS), 0, s, g, (const T *)x, ws, (T *)y, mean, rstd);
     else
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, false>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)x, ws, (T *)y, mean, rstd);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, false>), blocks, dim3(THREADS), 0, s, g, (const T *)x, ws, (T *)y, mean, rstd);
     return check_launch("group norm: launch failed");
 }
 
@@ -1110,15 +1142,17 @@ template <typename T, int V, bool SWISH>
 int backward_launch(const Geometry &g, const void *dy, const void *x, const float *mean, const float *rstd, void *dx, float *dgamma,
                     float *dbeta, float *dshift, float *ws, hipStream_t s)
 {
-    const int64_t blocks = g.batch * g.nchunk * g.ntile, rows = g.batch * g.nchunk, plane = rows * g.channels;
-    if (blocks > 0x7fffffff) return idm_set_error(IDM_ERR_INVALID, "group norm: batch too large");
-    hipLaunchKernelGGL((gn_grad_sums_kernel<T, V, SWISH>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)dy, (const T *)x, mean,
-                       rstd, ws, dshift != nullptr);
-    float *part = ws + 3 * plane, *per_sample = nullptr;
+    const int64_t rows = g.batch * g.nchunk, plane = rows * g.channels;
+    float2 *groups = (float2 *)ws;
+    float *sums = ws + 2 * rows * g.tpg * g.groups, *part = sums + 3 * plane, *per_sample = nullptr;
     if (dshift && g.shift_sample == 0) per_sample = part + (size_t)2 * kSplits * g.channels;   // one row for all samples: summed below
-    hipLaunchKernelGGL((gn_grad_apply_kernel<T, V, SWISH>), dim3((unsigned)blocks), dim3(THREADS), 0, s, g, (const T *)dy, (const T *)x, mean,
-                       rstd, (const float *)ws, (T *)dx, per_sample ? per_sample : dshift);
-    if (dbeta || dgamma) column_sums(ws, rows, g.channels, part, dbeta, dgamma, 2, s);
+    hipLaunchKernelGGL((gn_grad_sums_kernel<T, V, SWISH>), chunk_grid(g, 0), dim3(THREADS), 0, s, g, (const T *)dy, (const T *)x, mean, rstd,
+                       sums, groups, dshift != nullptr);
+    const bool here = (dbeta || dgamma) && rows <= 2048;   // few rows: the weight gradients in the same launch
+    hipLaunchKernelGGL((gn_grad_apply_kernel<T, V, SWISH>), chunk_grid(g, here ? (g.channels + 15) / 16 * 2 : 0), dim3(THREADS), 0, s, g,
+                       (const T *)dy, (const T *)x, mean, rstd, (const float *)sums, (const float2 *)groups, (T *)dx,
+                       per_sample ? per_sample : dshift, dbeta, dgamma);
+    if ((dbeta || dgamma) && !here) column_sums(sums, rows, g.channels, part, dbeta, dgamma, 2, s);
     if (per_sample) column_sums(per_sample, g.batch, g.channels, part, dshift, nullptr, 1, s);
     return check_launch("group norm backward: launch failed");
 }
