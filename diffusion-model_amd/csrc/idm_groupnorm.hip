@@ -60,6 +60,10 @@ template <int V> DEVI void load_chan(const float *p, int c, float missing, float
 
 DEVI float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
 
+// i / n from inv = 1 / n, for the small numbers of a workgroup (i < 2^13, n <= 2^10): (i + 1/2) * inv is off by less than 2^-10 / n, and the
+// nearest integer 1 / 2n away
+DEVI int quotient(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
+
 // Count, mean and sum of squared distances from it, of a set of values; join() is the union of two sets.  Sums of raw squares
 // would lose the variance of values that lie far from zero.
 struct Moments {
@@ -71,6 +75,32 @@ DEVI Moments join(const Moments &a, const Moments &b)
     if (n == 0.0f) return a;
     const float w = b.n / n, d = b.mean - a.mean;
     return {n, a.mean + d * w, a.m2 + b.m2 + d * d * (a.n * w)};
+}
+
+// The union of many sets, spread over `lanes` lanes: count and mean first, then the squared distances from that mean; no division but
+// one.  get(i) is set i.
+template <typename F> DEVI Moments join_all(int sets, int lane, int lanes, F &&get)
+{
+    float n = 0.0f, sum = 0.0f, m2 = 0.0f;
+#pragma unroll 4
+    for (int i = lane; i < sets; i += lanes) {
+        const Moments t = get(i);
+        n += t.n;
+        sum = __builtin_fmaf(t.n, t.mean, sum);
+    }
+    for (int off = lanes >> 1; off >= 1; off >>= 1) {
+        n += __shfl_xor(n, off, 64);
+        sum += __shfl_xor(sum, off, 64);
+    }
+    const float mean = sum / n;
+#pragma unroll 4
+    for (int i = lane; i < sets; i += lanes) {
+        const Moments t = get(i);
+        const float d = t.mean - mean;
+        m2 += __builtin_fmaf(t.n * d, d, t.m2);
+    }
+    for (int off = lanes >> 1; off >= 1; off >>= 1) m2 += __shfl_xor(m2, off, 64);
+    return {n, mean, m2};
 }
 
 // How the kernels cut a tensor.  A channel tile is at most THREADS vectors of V channels: gpt whole groups, or (groups wider
@@ -166,12 +196,12 @@ __global__ __launch_bounds__(THREADS) void gn_stats_kernel(Geometry g, const T *
     __syncthreads();
     // wavefront k joins groups k, k + 4, ...: entry e of a group is thread (e / qg) * q + group * qg + e % qg
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qg = q / w.ng, entries = rows * qg;
+    const float inv_qg = 1.0f / (float)qg;
     for (int k = wave; k < w.ng; k += THREADS / 64) {
-        Moments t = {0.0f, 0.0f, 0.0f};
-        for (int e = lane; e < entries; e += 64) t = join(t, sh[(e / qg) * q + k * qg + e % qg]);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1)
-            t = join(t, {__shfl_xor(t.n, off, 64), __shfl_xor(t.mean, off, 64), __shfl_xor(t.m2, off, 64)});
+        const Moments t = join_all(entries, lane, 64, [&](int e) {
+            const int er = quotient(e, inv_qg);
+            return sh[er * q + k * qg + e - er * qg];
+        });
         if (lane == 0) {
             const int part = g.tpg == 1 ? 0 : w.tile % g.tpg;
             float *o = partial + (((w.b * g.nchunk + w.chunk) * g.tpg + part) * g.groups + w.g0 + k) * 3;
@@ -197,17 +227,11 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
     const int lane = threadIdx.x & (lanes - 1);
     for (int k0 = 0; k0 < w.ng; k0 += THREADS / lanes) {
         const int k = k0 + (int)threadIdx.x / lanes;
-        Moments t = {0.0f, 0.0f, 0.0f};
-        if (k < w.ng) {
-            const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
-#pragma unroll 4
-            for (int i = lane; i < np; i += lanes) {
-                const float *o = pp + (int64_t)i * g.groups * 3;
-                t = join(t, {o[0], o[1], o[2]});
-            }
-        }
-        for (int off = lanes >> 1; off >= 1; off >>= 1)
-            t = join(t, {__shfl_xor(t.n, off, 64), __shfl_xor(t.mean, off, 64), __shfl_xor(t.m2, off, 64)});
+        const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
+        const Moments t = join_all(k < w.ng ? np : 0, lane, lanes, [&](int i) {
+            const float *o = pp + (int64_t)i * g.groups * 3;
+            return Moments{o[0], o[1], o[2]};
+        });
         if (k >= w.ng || lane) continue;
         const float rstd = 1.0f / sqrtf(t.m2 / t.n + g.eps);
         s_mean[k] = t.mean;
@@ -492,8 +516,7 @@ DEVI u32x4 load16(__amdgpu_buffer_rsrc_t b, int at) { return __builtin_amdgcn_ra
 DEVI void store16(__amdgpu_buffer_rsrc_t b, int at, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, at, 0, 0); }
 
 // A block is `pack` samples times one tile of ng groups; a sample's part is rows * q threads (`seats`), row r has pixels r, r + rows, ...:
-// full of them, one more where r < more.  Reciprocals instead of divisions: (i + 1/2) * (1 / n) cut to an integer is i / n for the
-// small numbers here (i < 2^13, n <= 2^10: the product is off by less than 2^-10 / n, the nearest integer is 1 / 2n away).
+// full of them, one more where r < more. 
 struct UnitArgs {
     int64_t batch, x_sample, x_pixel, dy_sample, dy_pixel, shift_sample;
     int pixels, channels, groups, gc, ng, q, qg, rows, full, more, seats, pack, swish;
@@ -506,7 +529,6 @@ DEVI float over(float s, float n, float r)
     const float m = s * r;
     return __builtin_fmaf(__builtin_fmaf(-m, n, s), r, m);
 }
-DEVI int quotient(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
 
 constexpr int kTileVecs = 64;   // vectors of a tile, unless one group (or the fewest whole groups that are whole vectors) is wider
 
