@@ -9,7 +9,8 @@ models.  Public surface mirrors the reference script's callables:
     onsager_energy …                          onsager.py
     bitflip.BitflipModel / bitflip.diffusion_backward
                                               mnist_diffusion.py: model([X, t]) and its XOR sampler
-    group_norm / adamw_step, AdamW            the norms and the optimizer step of its training
+    bitflip.BitflipTrainer                    its training loop, on group_norm and AdamW
+    group_norm / adamw_step, AdamW            the norms of that training and its optimizer step
 """
 from .keras_file import UNetSpec, load_unet_spec
 from .onsager import onsager_energy, onsager_heat_capacity, onsager_magnetization, theoretical_critical_kT

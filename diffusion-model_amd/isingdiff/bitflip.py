@@ -210,3 +210,100 @@ def diffusion_backward(X_b, model: BitflipModel, time_step: int | None = None, *
                                                   None if u is None else u.data_ptr(),
                                                   None if traj is None else traj.data_ptr(), B, H, W, model._stream()))
     return traj[..., None] if return_trajectory else x[..., None]
+
+
+class BitflipTrainer:
+    """Trains the weights of :class:`BitflipModel` (the reference's loop: ``mnist_diffusion.py:342-375``, binary cross-entropy of the
+    flip probabilities).
+
+        trainer = BitflipTrainer(synthetic_weights(0), device=0, time_step=100)
+        loss = trainer.step(X, t, flips)          # one AdamW step; loss is a 0-dim tensor on the GPU
+        model = trainer.model("bf16")             # a BitflipModel with the weights as they are now
+
+    X and flips are (B,H,W) 0/1 (the noisy images, and which of their bits to flip), t the step index of each sample.  The norms
+    (with the time vectors added on the way in) and the optimizer step run on this library's kernels, forward and backward; the
+    convolutions are torch matrix products over gathered 3x3 neighbourhoods.  ``precision="bf16"`` computes with bfloat16
+    activations and operands; weights, statistics, moments and gradients of weights stay float32.  Kernels (``*_w``) decay, offsets
+    and scales do not."""
+
+    def __init__(self, weights: dict, device: int = 0, time_step: int = 100, precision: str = "fp32", time_input: str = "float",
+                 lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-7, weight_decay: float = 0.0, moment_bits: int = 32):
+        import torch
+        from .optim import AdamW
+        if precision not in ("fp32", "bf16"):
+            raise ValueError("precision must be 'fp32' or 'bf16'")
+        shapes = tensor_shapes()
+        for name, shape in shapes.items():
+            if np.shape(weights[name]) != shape:
+                raise ValueError(f"{name}: expected shape {shape}, got {np.shape(weights[name])}")
+        self.torch, self.device, self.time_step, self.time_input = torch, device, time_step, time_input
+        self.dtype = torch.bfloat16 if precision == "bf16" else torch.float32
+        dev = f"cuda:{device}"
+        self.emb = torch.from_numpy(sinusoidal_table(time_step, time_input=time_input)).to(dev)
+        self.params = {n: torch.nn.Parameter(torch.tensor(np.asarray(weights[n], np.float32), device=dev)) for n in shapes}
+        self.opt = AdamW(self.params.values(), lr=lr, betas=betas, eps=eps, moment_bits=moment_bits,
+                         weight_decay=[weight_decay if n.endswith("_w") else 0.0 for n in self.params])
+
+    def _conv(self, x, name):
+        """'same' convolution without its offset, channels last."""
+        torch, w = self.torch, self.params[name].to(self.dtype)
+        if w.shape[0] == 3:
+            h, wd = x.shape[1:3]
+            p = torch.nn.functional.pad(x, (0, 0, 1, 1, 1, 1))
+            x = torch.cat([p[:, i:i + h, j:j + wd] for i in range(3) for j in range(3)], -1)
+        return (x.reshape(-1, x.shape[-1]) @ w.reshape(-1, w.shape[-1])).view(*x.shape[:3], -1)
+
+    def _block(self, i, x, temb):
+        from .norm import group_norm
+        torch, p = self.torch, self.params
+        silu = torch.nn.functional.silu
+        g = lambda k: p[f"b{i}_{k}"]  # noqa: E731
+        tvec = silu(temb @ g("t_w") + g("t_b")) + g("c1_b")     # the offset of the first convolution travels with the time vector
+        h = self._conv(group_norm(x, g("g1_g"), g("g1_b")), f"b{i}_c1_w")
+        h = self._conv(group_norm(h, g("g2_g"), g("g2_b"), shift=tvec), f"b{i}_c2_w") + g("c2_b").to(self.dtype)
+        if f"b{i}_s_w" in p:
+            x = self._conv(x, f"b{i}_s_w") + g("s_b").to(self.dtype)
+        return x + h
+
+    def logits(self, X, t):
+        """(B,H,W) float32: the flip probabilities before the sigmoid, with gradients for ``params``."""
+        torch, p = self.torch, self.params
+        dev = self.emb.device
+        X, t = torch.as_tensor(X).to(dev), torch.as_tensor(t)
+        if X.dim() != 3 or X.shape[1] % 4 or X.shape[2] % 4 or 0 in X.shape:
+            raise ValueError("X must be (B,H,W), H and W multiples of 4 (two 2x2 poolings)")
+        if t.shape != X.shape[:1] or t.dtype not in (torch.int32, torch.int64):
+            raise ValueError("t must be (B,) integers")
+        if int(t.min()) < 0 or int(t.max()) >= self.time_step:     # (waits for a t that is on the GPU)
+            raise ValueError(f"t must be in [0, {self.time_step})")
+        t = t.to(dev)
+        silu = torch.nn.functional.silu
+        temb = silu(self.emb[t.long()] @ p["d1_w"] + p["d1_b"])
+        temb = silu(temb @ p["d2_w"] + p["d2_b"])
+        x = (X[..., None].float() * p["in_w"].view(-1) + p["in_b"]).to(self.dtype)
+        pool = lambda a: a.unflatten(2, (-1, 2)).unflatten(1, (-1, 2)).amax((2, 4))  # noqa: E731
+        grow = lambda a: a.repeat_interleave(2, 1).repeat_interleave(2, 2)  # noqa: E731
+        s1 = self._block(0, x, temb)
+        s2 = self._block(1, pool(s1), temb)
+        mid = self._block(2, pool(s2), temb)
+        d3 = self._block(3, torch.cat([grow(mid), s2], -1), temb)
+        d4 = self._block(4, torch.cat([grow(d3), s1], -1), temb)
+        return d4.float() @ p["out_w"].view(-1) + p["out_b"]
+
+    def step(self, X, t, flips):
+        """One optimizer step on a batch; returns the mean cross-entropy before it."""
+        flips = self.torch.as_tensor(flips).to(self.emb.device).float()
+        logits = self.logits(X, t)
+        if flips.shape != logits.shape:
+            raise ValueError("flips must have the shape of X")
+        loss = self.torch.nn.functional.binary_cross_entropy_with_logits(logits, flips)
+        self.opt.zero_grad()
+        loss.backward()
+        self.opt.step()
+        return loss.detach()
+
+    def weights(self) -> dict:
+        return {n: p.detach().cpu().numpy().copy() for n, p in self.params.items()}
+
+    def model(self, precision: str = "fp32") -> BitflipModel:
+        return BitflipModel(self.weights(), self.device, self.time_step, precision, self.time_input)
