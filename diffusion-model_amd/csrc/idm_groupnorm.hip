@@ -1002,16 +1002,41 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
         return true;
     };
     bool ok = false;
+    if (backward) {
+        // The share of the wavefronts that a compute unit can hold (the registers allow 8 or 12, float32 12 or 16) that hold values, times
+        // how much of the chip has a block; parts of a pixel that are no whole 64 bytes, and a block alone on its compute unit,
+        // cost some (1 024 x 14 x 14 x 192 bf16: 0.77 of the seats full in tiles of 192 bytes 59 us, in tiles of 48 bytes 67 us, 0.57 full
+        // 65 - 69 us).
+        float best = 0.0f;
+        UnitPlan chosen = u;
+        for (int i = 0; i < 2; ++i)
+            for (int tiles = 1; tiles <= units; ++tiles) {
+                if (!fits(tiles, i)) continue;
+                const int room = (i == 0 ? 8 : 12) + (e == 4 && u.pieces == 1 ? 4 : 0), waves = u.threads / 64, blocks = room / waves;
+                if (!blocks) continue;
+                const int64_t packs = (d.batch + u.pack - 1) / u.pack, part = (int64_t)u.q * 16;
+                float use = (float)(u.rows * u.q * u.pack) / (float)u.threads * (float)d.pixels / (float)(u.rows * u.nv) * (float)(blocks * waves) / (float)room;
+                use *= std::min(1.0f, (float)(packs * tiles) / (256.0f * (float)blocks));
+                use *= (part % 64 == 0 ? 1.0f : part % 32 == 0 ? 0.96f : 0.85f) * (blocks == 1 ? 0.95f : 1.0f);
+                if (use > best) {
+                    best = use;
+                    chosen = u;
+                    chosen.walkers = std::max(1, 256 * blocks / tiles);   // one more would be a second turn of the chip
+                }
+            }
+        u = chosen;
+        return best > 0.0f && walkers(u.walkers);
+    }
     // The narrowest tile of whole 64-byte parts that makes 256 blocks: narrow ones leave several blocks to a compute unit, one of which
     // loads while another computes; parts of 48 or 32 bytes cost a third of the bandwidth (1 024 x 28 x 28 x 96 bf16, forward: tiles of
     // 32 / 64 / 96 / 192 bytes 85 / 67 / 75 / 75 us).  With fewer samples the chip fills first: narrower tiles.
-    for (int i = 0; i < (backward ? 1 : 2) && !ok; ++i)
+    for (int i = 0; i < 2 && !ok; ++i)
         for (int tiles = units; tiles >= 1 && !ok; --tiles) ok = units % tiles == 0 && units / tiles * wide % 4 == 0 && d.batch * tiles >= 256 && fits(tiles, i);
     for (int i = 0; i < 2 && !ok; ++i)
         for (int tiles = 1; tiles <= units && !ok; ++tiles) ok = d.batch * tiles >= 256 && fits(tiles, i);
     for (int i = 0; i < 2 && !ok; ++i) ok = fits(units, i) && (u.threads <= 512 || d.batch * units >= 128);
     if (!ok) return false;
-    return walkers((256 * 1024 / u.threads + u.tiles - 1) / u.tiles);
+    return true;
 }
 
 // What a call needs.  Unless the caller says that all pointers are aligned, the size query does not know which form and vector width
