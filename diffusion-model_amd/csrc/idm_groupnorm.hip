@@ -996,47 +996,45 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
         u.pack = (int)pack;
         return true;
     };
-    auto walkers = [&](int64_t want) {
-        const int64_t packs = (d.batch + u.pack - 1) / u.pack, turns = (packs + want - 1) / want;
-        u.walkers = (packs + turns - 1) / turns;
-        return true;
-    };
-    bool ok = false;
-    if (backward) {
-        // The share of the wavefronts that a compute unit can hold (the registers allow 8 or 12, float32 12 or 16) that hold values, times
-        // how much of the chip has a block; parts of a pixel that are no whole 64 bytes, and a block alone on its compute unit,
-        // cost some (1 024 x 14 x 14 x 192 bf16: 0.77 of the seats full in tiles of 192 bytes 59 us, in tiles of 48 bytes 67 us, 0.57 full
-        // 65 - 69 us).
-        float best = 0.0f;
-        UnitPlan chosen = u;
-        for (int i = 0; i < 2; ++i)
-            for (int tiles = 1; tiles <= units; ++tiles) {
-                if (!fits(tiles, i)) continue;
-                const int room = (i == 0 ? 8 : 12) + (e == 4 && u.pieces == 1 ? 4 : 0), waves = u.threads / 64, blocks = room / waves;
-                if (!blocks) continue;
-                const int64_t packs = (d.batch + u.pack - 1) / u.pack, part = (int64_t)u.q * 16;
-                float use = (float)(u.rows * u.q * u.pack) / (float)u.threads * (float)d.pixels / (float)(u.rows * u.nv) * (float)(blocks * waves) / (float)room;
-                use *= std::min(1.0f, (float)(packs * tiles) / (256.0f * (float)blocks));
-                use *= (part % 64 == 0 ? 1.0f : part % 32 == 0 ? 0.96f : 0.85f) * (blocks == 1 ? 0.95f : 1.0f);
+    // The best of all tiles and instances by what part of the chip's time they use, estimated as the product of
+    //  - the seats that hold values (rows are cut to whole wavefronts, the last vector of a thread may be empty);
+    //  - the wavefronts at work: a block takes ceil(waves / 4) of a SIMD's places (forward 6 with 8 vectors, 4 with 16, 8 with 4; backward 2
+    //    and 3, float32 3 and 4); 16 of them (backward 8) keep the memory busy; a block alone loads, computes and stores in turn;
+    //  - what a thread does besides its vectors (a fifth more with 4 of them; 16 leave fewer wavefronts);
+    //  - the parts of a pixel: blocks of one sample share its 128-byte lines, and parts that are no whole 32 bytes share sectors too;
+    //  - blocks for all compute units, and whole turns of the walkers.
+    // Measured on three sets in turn, us, bf16: forward 1 024 x 784 x 96 in 12-channel groups, tiles of 48 / 96 / 192 bytes 83 / 77 / 83;
+    // 1 024 x 784 x 64, tiles of 32 / 64 / 128 bytes 55 / 44 / 49; backward 1 024 x 196 x 192, tiles of 48 / 96 / 192 bytes 79 / 76 / 69,
+    // 4 096 x 49 x 128, tiles of 32 / 64 / 128 bytes 62 / 47 / 45.
+    const int64_t pixel = (int64_t)d.channels * e;
+    float best = 0.0f;
+    UnitPlan chosen = u;
+    for (int i = 0; i < (backward ? 2 : 3); ++i)
+        for (int tiles = 1; tiles <= units; ++tiles) {
+            if (!fits(tiles, i)) continue;
+            const int waves = u.threads / 64, many = backward ? 8 : 16;
+            const int places = backward ? (i == 0 ? 2 : 3) + (e == 4 && u.pieces == 1) : u.nv == 8 ? 6 : u.nv == 16 ? 4 : 8;
+            const int most = waves < 4 ? places * 4 / waves : places / ((waves + 3) / 4);
+            const int64_t packs = (d.batch + u.pack - 1) / u.pack, part = (int64_t)u.q * 16;
+            const float seats = (float)(u.rows * u.q * u.pack) / (float)u.threads * (float)d.pixels / (float)(u.rows * u.nv);
+            const float shared = (float)std::min<int64_t>(128, pixel) / (float)part;
+            const float lines = std::max(0.5f, shared > 1.0f ? 1.0f - 0.06f * (shared - 1.0f) : 1.0f) * (part % 32 ? 0.85f : 1.0f);
+            for (int blocks = backward ? 1 : most; blocks <= most; ++blocks) {
+                float use = seats * lines * std::min(1.0f, (float)(blocks * waves) / (float)many) * (blocks > 1 + !backward ? 1.0f : blocks > 1 ? 0.97f : backward ? 0.9f : 0.85f) *
+                            (u.nv == 4 ? 0.8f : u.nv == 16 ? 0.95f : 1.0f);
+                use *= std::min(1.0f, (float)(packs * tiles) / 256.0f);
+                const int64_t want = std::max(1, 256 * blocks / tiles), turns = (packs + want - 1) / want, n = (packs + turns - 1) / turns;
+                if (backward) use *= (float)packs / (float)(turns * std::min(want, packs));
                 if (use > best) {
                     best = use;
                     chosen = u;
-                    chosen.walkers = std::max(1, 256 * blocks / tiles);   // one more would be a second turn of the chip
+                    chosen.walkers = n;
                 }
             }
-        u = chosen;
-        return best > 0.0f && walkers(u.walkers);
-    }
-    // The narrowest tile of whole 64-byte parts that makes 256 blocks: narrow ones leave several blocks to a compute unit, one of which
-    // loads while another computes; parts of 48 or 32 bytes cost a third of the bandwidth (1 024 x 28 x 28 x 96 bf16, forward: tiles of
-    // 32 / 64 / 96 / 192 bytes 85 / 67 / 75 / 75 us).  With fewer samples the chip fills first: narrower tiles.
-    for (int i = 0; i < 2 && !ok; ++i)
-        for (int tiles = units; tiles >= 1 && !ok; --tiles) ok = units % tiles == 0 && units / tiles * wide % 4 == 0 && d.batch * tiles >= 256 && fits(tiles, i);
-    for (int i = 0; i < 2 && !ok; ++i)
-        for (int tiles = 1; tiles <= units && !ok; ++tiles) ok = d.batch * tiles >= 256 && fits(tiles, i);
-    for (int i = 0; i < 2 && !ok; ++i) ok = fits(units, i) && (u.threads <= 512 || d.batch * units >= 128);
-    if (!ok) return false;
-    return true;
+        }
+    u = chosen;
+    // few large units: the form that cuts a sample into chunks fills the chip
+    return best > 0.1f || (best > 0.0f && d.pixels * u.q * 16 <= 65536);
 }
 
 // What a call needs.  Unless the caller says that all pointers are aligned, the size query does not know which form and vector width
