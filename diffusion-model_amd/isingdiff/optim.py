@@ -84,11 +84,17 @@ def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), ep
     where = set(map(Tensor.get_device, params)) | set(map(Tensor.get_device, given))
     if {p.dtype for p in params} != {ptype} or len(where) != 1 or not all(map(Tensor.is_contiguous, params)):
         raise ValueError("parameters must be dense, of one type and on one device")
-    if given and ({g.dtype for g in given} != {gtype} or list(map(Tensor.size, given)) != list(map(Tensor.size, with_grad))):
-        raise ValueError("a gradient must have its parameter's shape and device, and all gradients one type")
+    if given and {g.dtype for g in given} != {gtype}:
+        raise ValueError("all gradients must be of one type")
     if not all(map(Tensor.is_contiguous, given)):
         given = [g.contiguous() for g in given]
-    sizes = array("q", map(Tensor.numel, params))
+    counts = list(map(Tensor.numel, params))
+    sizes = array("q", counts)
+    # (dense tensors of the same strides and sizes hold the same entries in the same order; shapes cost more to ask for)
+    same = (list(map(Tensor.stride, given)) == list(map(Tensor.stride, with_grad))
+            and list(map(Tensor.numel, given)) == (counts if with_grad is params else list(map(Tensor.numel, with_grad))))
+    if not same and [g.shape for g in given] != [p.shape for p in with_grad]:
+        raise ValueError("a gradient must have its parameter's shape and device")
     if isinstance(weight_decay, (int, float)):
         lowest, decay = weight_decay, array("f", (weight_decay,)) * n
     else:
@@ -99,12 +105,12 @@ def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), ep
     if not (math.isfinite(lr) and lr >= 0 and math.isfinite(eps) and eps >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1
             and lowest >= 0 and math.isfinite(sum(decay))):
         raise ValueError("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)")
-    bits = _check_state(state, sum([s + BLOCK - 1 >> 8 for s in sizes]) * BLOCK, dev)
+    bits = _check_state(state, sum([s + BLOCK - 1 >> 8 for s in counts]) * BLOCK, dev)
     if dev.type != "cuda":
         raise ValueError("parameters must be CUDA tensors")
-    at = array("q", map(Tensor.data_ptr, params))
-    if given is grads or len(given) == n:
-        grad_at = array("q", map(Tensor.data_ptr, given))
+    at = array("q", list(map(Tensor.data_ptr, params)))
+    if len(given) == n:
+        grad_at = array("q", list(map(Tensor.data_ptr, given)))
     else:
         it = iter(given)
         grad_at = array("q", [0 if g is None else next(it).data_ptr() for g in grads])
@@ -115,9 +121,7 @@ def adamw_step(params, grads, state, *, lr: float = 1e-3, betas=(0.9, 0.999), ep
                                             decay.buffer_info()[0], state["m"].data_ptr(), state["v"].data_ptr(), *base,
                                             state["m"].numel(), state["step"].data_ptr(), scratch.data_ptr()))
     # the kernel writes behind autograd's back: a backward pass that saved a parameter has to see that it changed
-    leaves = [p for p in params if p.requires_grad]
-    if leaves:
-        torch.autograd.graph.increment_version(leaves)
+    torch.autograd.graph.increment_version(params)
 
 
 def adamw_moments(state):
