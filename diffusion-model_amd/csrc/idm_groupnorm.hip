@@ -543,27 +543,27 @@ template <int V> DEVI void load_chan16(const float *p, int c, float missing, flo
     }
 }
 
-// sum += the vector's values, squares += their squares, both in float32 from pairs
-DEVI void add_pairs(u32x4 raw, _Float16, float &sum, float &squares)
+// sum += the values of each of a vector's P pieces (1 or 2), squares += their squares, both in float32 and two values at a time
+template <int P> DEVI void add_pairs(u32x4 raw, _Float16, float sum[P], float squares[P])
 {
     typedef __attribute__((ext_vector_type(2))) _Float16 half2_;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const unsigned w = raw[j];   // (a copy: the cast of an element itself takes the first one)
         const half2_ v = __builtin_bit_cast(half2_, w);
-        sum = __builtin_amdgcn_fdot2(v, half2_{1, 1}, sum, false);
-        squares = __builtin_amdgcn_fdot2(v, v, squares, false);
+        sum[j * P / 4] = __builtin_amdgcn_fdot2(v, half2_{1, 1}, sum[j * P / 4], false);
+        squares[j * P / 4] = __builtin_amdgcn_fdot2(v, v, squares[j * P / 4], false);
     }
 }
-DEVI void add_pairs(u32x4 raw, __bf16, float &sum, float &squares)
+template <int P> DEVI void add_pairs(u32x4 raw, __bf16, float sum[P], float squares[P])
 {
     typedef __attribute__((ext_vector_type(2))) __bf16 bf2;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const unsigned w = raw[j];
         const bf2 v = __builtin_bit_cast(bf2, w);
-        sum = __builtin_amdgcn_fdot2_f32_bf16(v, bf2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
-        squares = __builtin_amdgcn_fdot2_f32_bf16(v, v, squares, false);
+        sum[j * P / 4] = __builtin_amdgcn_fdot2_f32_bf16(v, bf2{(__bf16)1.0f, (__bf16)1.0f}, sum[j * P / 4], false);
+        squares[j * P / 4] = __builtin_amdgcn_fdot2_f32_bf16(v, v, squares[j * P / 4], false);
     }
 }
 
@@ -646,14 +646,20 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
     // values instead of eight) stand: that loses less than five bits.
     const float own = (float)(s.mine ? s.mine * PS : 1), share = __builtin_amdgcn_rcpf(own);
     bool sure = false;
-    if constexpr (E == 2 && P == 1) {
+    if constexpr (E == 2 && P <= 2) {
         if (!g.shift) {
-            float sum = 0.0f, squares = 0.0f;
+            float sum[P], squares[P];
 #pragma unroll
-            for (int k = 0; k < NV; ++k) add_pairs(raw[k], T{}, sum, squares);
-            mean[0] = over(sum, own, share);
-            m2[0] = squares - sum * mean[0];
-            sure = !(m2[0] * 16.0f < sum * mean[0]);
+            for (int i = 0; i < P; ++i) sum[i] = squares[i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) add_pairs<P>(raw[k], T{}, sum, squares);
+            sure = true;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                mean[i] = over(sum[i], own, share);
+                m2[i] = squares[i] - sum[i] * mean[i];
+                sure = sure && !(m2[i] * 16.0f < sum[i] * mean[i]);
+            }
         }
     }
     if (!sure) {
@@ -999,7 +1005,7 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
     // The best of all tiles and instances by what part of the chip's time they use, estimated as the product of
     //  - the seats that hold values (rows are cut to whole wavefronts, the last vector of a thread may be empty);
     //  - the wavefronts at work: a block takes ceil(waves / 4) of a SIMD's places (forward 6 with 8 vectors, 4 with 16, 8 with 4; backward 2
-    //    and 3, float32 3 and 4); 16 of them (backward 8) keep the memory busy; a block alone loads, computes and stores in turn;
+    //    and 3, float32 3 and 4); 12 of them (backward 8) keep the memory busy; a block alone loads, computes and stores in turn;
     //  - what a thread does besides its vectors (a fifth more with 4 of them; 16 leave fewer wavefronts);
     //  - the parts of a pixel: blocks of one sample share its 128-byte lines, and parts that are no whole 32 bytes share sectors too;
     //  - blocks for all compute units, and whole turns of the walkers.
@@ -1012,7 +1018,7 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
     for (int i = 0; i < (backward ? 2 : 3); ++i)
         for (int tiles = 1; tiles <= units; ++tiles) {
             if (!fits(tiles, i)) continue;
-            const int waves = u.threads / 64, many = backward ? 8 : 16;
+            const int waves = u.threads / 64, many = backward ? 8 : 12;
             const int places = backward ? (i == 0 ? 2 : 3) + (e == 4 && u.pieces == 1) : u.nv == 8 ? 6 : u.nv == 16 ? 4 : 8;
             const int most = waves < 4 ? places * 4 / waves : places / ((waves + 3) / 4);
             const int64_t packs = (d.batch + u.pack - 1) / u.pack, part = (int64_t)u.q * 16;
@@ -1033,8 +1039,9 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
             }
         }
     u = chosen;
-    // few large units: the form that cuts a sample into chunks fills the chip
-    return best > 0.1f || (best > 0.0f && d.pixels * u.q * 16 <= 65536);
+    // Few large units: the form that cuts a sample into chunks fills the chip (16 x 4 096 x 64 bf16, backward: 19.6 us against 23.6;
+    // 16 x 16 384 x 32 float32, forward: 26 against 41).  Small units are done before its second launch has begun.
+    return best > (backward ? 0.5f : 0.3f) || (best > 0.0f && d.pixels * u.q * 16 <= (backward ? 40960 : 65536));
 }
 
 // What a call needs.  Unless the caller says that all pointers are aligned, the size query does not know which form and vector width
