@@ -8,11 +8,19 @@
 //   dx = rstd * (dz * gamma - A - xhat * B)   A = mean over the group of dz * gamma, B = of dz * gamma * xhat
 //   dshift[b, c] = sum over the pixels of dx = rstd * (gamma * sum dz - pixels * A - B * sum xhat)
 //
-// All arithmetic between the load and the store is float32; y and dx are rounded once, to the type of x.
+// All arithmetic between the load and the store is float32; y and dx are rounded once, to the type of x.  Sums run in a fixed order,
+// no atomics: equal inputs give equal bits.
 //
-// Two launches per direction: partial statistics of (sample, pixel chunk, channel tile), then a kernel that joins a sample's
-// partials and applies.  The weight gradients are partial sums per (sample, chunk) joined by two more small launches, in a
-// fixed order: no atomics, so results do not depend on the order in which workgroups run.
+// Memory bounds both directions: x in, y out (forward), x and dy in, dx out (backward); a large copy on this card moves 4.9 TB/s.  Next
+// comes the vector unit: a value costs about 15 of its slots forward (exp and rcp are four each) and 25 backward, a third to two
+// thirds of the time of its memory.  Two forms:
+//   units   one launch; a workgroup holds a channel tile of one sample (or of several small ones) in registers, so memory is touched
+//           once.  Backward adds a small launch for the weight gradients.  Forward 1 024 x 28 x 28 x 96 bf16: 79 us (3.9 TB/s; 105 in
+//           chunks); 4 096 x 7 x 7 x 128 bf16 22 us (4.7 TB/s; 42); backward 1 024 x 14 x 14 x 192 bf16: 73 us (3.2 TB/s; 93).
+//   chunks  two launches over chunks of pixels: partial sums, then their join and the result; x (and dy) are read twice, the second
+//           time mostly from the caches.  For maps that a compute unit cannot hold, few large ones, and calls whose pointers, strides
+//           or channels are no multiples of 16 bytes.  4 x 128 x 128 x 64 fp16: 14 us forward; 3 x 127 x 125 x 64 fp16: 16 us backward.
+// plan_unit() chooses.
 #include "../../include/isingdiff.h"
 #include "idm_internal.h"
 #include "idm_device.h"
@@ -144,7 +152,10 @@ DEVI Place place_of(const Geometry &g, int part_channels)
     return w;
 }
 
-// Partial statistics: partial[(b * nchunk + chunk) * tpg + part][group] = (n, mean, m2) as three planes' worth of floats.
+// ---- chunks ---------------------------------------------------------------------------------------------------------------
+//
+// Partial statistics of (sample, chunk, tile): (n, mean, m2) of each group at ((b * nchunk + chunk) * tpg + part) * groups + group.  Chunks
+// of at least four vectors a thread, enough of them for 2 048 workgroups.
 template <typename T, int V>
 __global__ __launch_bounds__(THREADS) void gn_stats_kernel(Geometry g, const T *__restrict__ x, float *__restrict__ partial)
 {
@@ -516,7 +527,7 @@ DEVI u32x4 load16(__amdgpu_buffer_rsrc_t b, int at) { return __builtin_amdgcn_ra
 DEVI void store16(__amdgpu_buffer_rsrc_t b, int at, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, at, 0, 0); }
 
 // A block is `pack` samples times one tile of ng groups; a sample's part is rows * q threads (`seats`), row r has pixels r, r + rows, ...:
-// full of them, one more where r < more. 
+// full of them, one more where r < more.
 struct UnitArgs {
     int64_t batch, x_sample, x_pixel, dy_sample, dy_pixel, shift_sample;
     int pixels, channels, groups, gc, ng, q, qg, rows, full, more, seats, pack, swish;
@@ -658,7 +669,7 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
             for (int i = 0; i < P; ++i) {
                 mean[i] = over(sum[i], own, share);
                 m2[i] = squares[i] - sum[i] * mean[i];
-                sure = sure && !(m2[i] * 16.0f < sum[i] * mean[i]);
+                sure = sure && squares[i] < 0x1p126f && !(m2[i] * 16.0f < sum[i] * mean[i]);   // (squares that overflow, too)
             }
         }
     }
@@ -1016,7 +1027,7 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
     float best = 0.0f;
     UnitPlan chosen = u;
     for (int i = 0; i < (backward ? 2 : 3); ++i)
-        for (int tiles = 1; tiles <= units; ++tiles) {
+        for (int tiles = 1; tiles <= std::min(units, 4096); ++tiles) {
             if (!fits(tiles, i)) continue;
             const int waves = u.threads / 64, many = backward ? 8 : 12;
             const int places = backward ? (i == 0 ? 2 : 3) + (e == 4 && u.pieces == 1) : u.nv == 8 ? 6 : u.nv == 16 ? 4 : 8;

@@ -123,6 +123,20 @@ def test_against_the_formula(shape, groups, dtype):
     verify(x, gamma, beta, shift, dy, groups, "swish" if n % 3 else "none")
 
 
+# batches that the forms for many samples take: several samples to a block, several turns of a block, a last pack that is not full,
+# groups that straddle vectors (5, 6, 12, 1 channels), one pixel, rows that are not full
+MANY = [((70, 6, 6, 40), 8), ((1501, 3, 3, 16), 4), ((90, 14, 14, 192), 8), ((65, 28, 28, 96), 8), ((2051, 1, 1, 64), 8), ((777, 7, 7, 48), 8),
+        ((130, 5, 13, 64), 64), ((300, 9, 9, 128), 32), ((513, 2, 1, 8), 1), ((70, 25, 41, 32), 8)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,groups", MANY)
+def test_many_samples(shape, groups, dtype):
+    n = sum(shape) + groups
+    x, gamma, beta, shift, dy = inputs(shape, TYPES[dtype], n, groups, shift=["rows", "none", "one", "none"][n % 4])
+    verify(x, gamma, beta, shift, dy, groups, "swish" if n % 3 else "none")
+
+
 @pytest.mark.parametrize("act", ["swish", "none"])
 @pytest.mark.parametrize("shift", ["rows", "one", "flat", "none"])
 def test_activation_and_shift(act, shift):
@@ -135,6 +149,30 @@ def test_values_far_from_zero():
     x, gamma, beta, _, dy = inputs((2, 40, 40, 16), torch.float32, 11, 4)
     x = x + 1000.0
     verify(x, gamma, beta, None, dy, 4, "swish")
+
+
+def test_a_variance_beyond_float32():
+    """Deviations of at least 2^61 (2^62 times half a unit): the squares of a group's 20 * 20 * 8 values add up to more than 3 200 * 2^122 =
+    2^133, and float32 ends below 2^128.  The sum is infinite, so rstd is zero and y = act(beta); the mean is right."""
+    from isingdiff import group_norm_forward
+    x, gamma, beta, _, dy = inputs((3, 20, 20, 64), torch.bfloat16, 41, 8, shift="none")
+    x = (x.float() * 2.0 ** 62 + 2.0 ** 66).to(torch.bfloat16)
+    y, mean, rstd = group_norm_forward(x, gamma, beta, 8, eps=0.0)
+    w = exact(x, gamma, beta, None, 8, 0.0, "swish")
+    check("mean", mean, w["mean"], 64 * E * w["k"] / w["rstd"])
+    assert not rstd.any()
+    want = (beta.double() * torch.sigmoid(beta.double())).cpu().expand(y.shape)
+    check("y", y, want, half_step(torch.bfloat16) * want.abs() + 16 * E)
+
+
+@pytest.mark.parametrize("scale,offset", [(1.0, 100.0), (2.0 ** 40, 0.0), (2.0 ** 56, 2.0 ** 64)])
+def test_bfloat16_far_from_zero_and_large(scale, offset):
+    """Means of many deviations, and values whose squares leave float32 while those of the deviations do not: the short way over sums
+    of squares has to give up by itself."""
+    x, gamma, beta, _, dy = inputs((3, 20, 20, 64), torch.bfloat16, 41, 8, shift="none")
+    verify((x.float() * scale + offset).to(torch.bfloat16), gamma, beta, None, dy, 8, "swish", eps=0.0)
+    x, gamma, beta, _, dy = inputs((3, 20, 20, 32), torch.bfloat16, 42, 8, shift="none")
+    verify((x.float() * scale + offset).to(torch.bfloat16), gamma, beta, None, dy, 8, "none", eps=0.0)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
