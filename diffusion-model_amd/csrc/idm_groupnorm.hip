@@ -35,10 +35,8 @@ constexpr int THREADS = 256;
 template <typename T, int V> struct VecOf { typedef __attribute__((ext_vector_type(V))) T type; };
 template <typename T> struct VecOf<T, 1> { typedef T type; };
 
-// V consecutive channels as float32
-template <typename T, int V> DEVI void load_vec(const T *p, float out[V])
+template <typename T, int V> DEVI void widen_vec(const typename VecOf<T, V>::type &v, float out[V])
 {
-    const typename VecOf<T, V>::type v = *(const typename VecOf<T, V>::type *)p;
     if constexpr (V == 1) {
         out[0] = (float)v;
     } else {
@@ -46,6 +44,9 @@ template <typename T, int V> DEVI void load_vec(const T *p, float out[V])
         for (int j = 0; j < V; ++j) out[j] = (float)v[j];
     }
 }
+
+// V consecutive channels as float32
+template <typename T, int V> DEVI void load_vec(const T *p, float out[V]) { widen_vec<T, V>(*(const typename VecOf<T, V>::type *)p, out); }
 
 template <typename T, int V> DEVI void store_vec(T *p, const float in[V])
 {
@@ -71,6 +72,13 @@ DEVI float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdg
 // i / n from inv = 1 / n, for the small numbers of a workgroup (i < 2^13, n <= 2^10): (i + 1/2) * inv is off by less than 2^-10 / n, and the
 // nearest integer 1 / 2n away
 DEVI int quotient(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
+
+// s / n with r near 1 / n: exact wherever the quotient is a float (a constant group's mean is its value)
+DEVI float over(float s, float n, float r)
+{
+    const float m = s * r;
+    return __builtin_fmaf(__builtin_fmaf(-m, n, s), r, m);
+}
 
 // Count, mean and sum of squared distances from it, of a set of values; join() is the union of two sets.  Sums of raw squares
 // would lose the variance of values that lie far from zero.
@@ -154,8 +162,8 @@ DEVI Place place_of(const Geometry &g, int part_channels)
 
 // ---- chunks ---------------------------------------------------------------------------------------------------------------
 //
-// Partial statistics of (sample, chunk, tile): (n, mean, m2) of each group at ((b * nchunk + chunk) * tpg + part) * groups + group.  Chunks
-// of at least four vectors a thread, enough of them for 2 048 workgroups.
+// Partial statistics of (sample, chunk, tile): (n, mean, m2) of each group at ((b * groups + group) * nchunk + chunk) * tpg + part,
+// so that the lanes which join a group read neighbours.
 template <typename T, int V>
 __global__ __launch_bounds__(THREADS) void gn_stats_kernel(Geometry g, const T *__restrict__ x, float *__restrict__ partial)
 {
@@ -214,8 +222,8 @@ __global__ __launch_bounds__(THREADS) void gn_stats_kernel(Geometry g, const T *
             return sh[er * q + k * qg + e - er * qg];
         });
         if (lane == 0) {
-            const int part = g.tpg == 1 ? 0 : w.tile % g.tpg;
-            float *o = partial + (((w.b * g.nchunk + w.chunk) * g.tpg + part) * g.groups + w.g0 + k) * 3;
+            const int part = g.tpg == 1 ? 0 : w.tile % g.tpg, np = g.nchunk * g.tpg;
+            float *o = partial + ((w.b * g.groups + w.g0 + k) * np + w.chunk * g.tpg + part) * 3;
             o[0] = t.n;
             o[1] = t.mean;
             o[2] = t.m2;
@@ -238,9 +246,9 @@ __global__ __launch_bounds__(THREADS) void gn_apply_kernel(Geometry g, const T *
     const int lane = threadIdx.x & (lanes - 1);
     for (int k0 = 0; k0 < w.ng; k0 += THREADS / lanes) {
         const int k = k0 + (int)threadIdx.x / lanes;
-        const float *pp = partial + (w.b * np * g.groups + w.g0 + k) * 3;
+        const float *pp = partial + (w.b * g.groups + w.g0 + k) * np * 3;
         const Moments t = join_all(k < w.ng ? np : 0, lane, lanes, [&](int i) {
-            const float *o = pp + (int64_t)i * g.groups * 3;
+            const float *o = pp + i * 3;
             return Moments{o[0], o[1], o[2]};
         });
         if (k >= w.ng || lane) continue;
@@ -302,6 +310,26 @@ DEVI void sum_columns(const float *in, int64_t rows, int cols, int col0, int spl
 #pragma unroll
             for (int k = 0; k < w; ++k) t[k] += t[k + w];
         out[(int64_t)split * cols + col] = t[0];
+    }
+}
+
+constexpr int kLoads = 4;
+
+// Calls use(p, vectors of x, vectors of dy) for a thread's pixels p, p + rows, ... (kLoads of them, below p1).  The last ones are loaded
+// together as well, with the first in place of those behind the end: a loop of single loads for them took 56 of 80 us on 300 x 28 x 28 x
+// 96 bf16.
+template <typename T, int V, typename F>
+DEVI void for_pixels(const Place &w, int r, int rows, const T *x, int64_t xpitch, const T *dy, int64_t dpitch, F &&use)
+{
+    for (int64_t p = w.p0 + r; p < w.p1; p += kLoads * (int64_t)rows) {
+        typename VecOf<T, V>::type u[kLoads], d[kLoads];
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            const int64_t at = p + k * (int64_t)rows, from = at < w.p1 ? at : p;
+            u[k] = *(const typename VecOf<T, V>::type *)(x + from * xpitch);
+            d[k] = *(const typename VecOf<T, V>::type *)(dy + from * dpitch);
+        }
+        use(p, u, d);
     }
 }
 
@@ -368,19 +396,22 @@ __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const
 #pragma unroll
         for (int j = 0; j < V; ++j) add[j] -= mean;
         const T *xp = x + w.b * g.x_sample + c, *dp = dy + w.b * g.dy_sample + c;
-#pragma unroll 4
-        for (int64_t p = w.p0 + r; p < w.p1; p += rows) {
-            float u[V], d[V], xhat[V], dz[V];
-            load_vec<T, V>(xp + p * g.x_pixel, u);
-            load_vec<T, V>(dp + p * g.dy_pixel, d);
-            grad_z<V, SWISH>(u, d, add, rstd, gamma, beta, xhat, dz);
+        for_pixels<T, V>(w, r, rows, xp, g.x_pixel, dp, g.dy_pixel, [&](int64_t p, auto &raw, auto &up) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                acc[0][j] += dz[j];
-                acc[1][j] = __builtin_fmaf(dz[j], xhat[j], acc[1][j]);
-                acc[2][j] += xhat[j];
+            for (int k = 0; k < kLoads; ++k) {
+                if (p + k * (int64_t)rows >= w.p1) continue;
+                float u[V], d[V], xhat[V], dz[V];
+                widen_vec<T, V>(raw[k], u);
+                widen_vec<T, V>(up[k], d);
+                grad_z<V, SWISH>(u, d, add, rstd, gamma, beta, xhat, dz);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    acc[0][j] += dz[j];
+                    acc[1][j] = __builtin_fmaf(dz[j], xhat[j], acc[1][j]);
+                    acc[2][j] += xhat[j];
+                }
             }
-        }
+        });
     }
     const int64_t plane = g.batch * g.nchunk * g.channels, row = (w.b * g.nchunk + w.chunk) * g.channels;
     for (int i = 0; i < (with_xhat ? 3 : 2); ++i) {
@@ -401,7 +432,7 @@ __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const
             t.x += by_channel[0][c];
             t.y += by_channel[1][c];
         }
-        groups[((w.b * g.nchunk + w.chunk) * g.tpg + part) * g.groups + w.g0 + k] = t;
+        groups[(w.b * g.groups + w.g0 + k) * (g.nchunk * g.tpg) + w.chunk * g.tpg + part] = t;
     }
 }
 
@@ -433,10 +464,10 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
         const int k = k0 + (int)threadIdx.x / lanes;
         float2 t = {0.0f, 0.0f};
         if (k < w.ng) {
-            const float2 *pp = groups + w.b * np * g.groups + w.g0 + k;
+            const float2 *pp = groups + (w.b * g.groups + w.g0 + k) * np;
 #pragma unroll 4
             for (int i = lane; i < np; i += lanes) {
-                const float2 o = pp[(int64_t)i * g.groups];
+                const float2 o = pp[i];
                 t.x += o.x;
                 t.y += o.y;
             }
@@ -476,16 +507,19 @@ __global__ __launch_bounds__(THREADS) void gn_grad_apply_kernel(Geometry g, cons
     for (int j = 0; j < V; ++j) add[j] -= mean;
     const T *xp = x + w.b * g.x_sample + c, *dp = dy + w.b * g.dy_sample + c;
     T *op = dx + w.b * g.pixels * g.channels + c;
-#pragma unroll 4
-    for (int64_t p = w.p0 + r; p < w.p1; p += rows) {
-        float u[V], d[V], xhat[V], dz[V];
-        load_vec<T, V>(xp + p * g.x_pixel, u);
-        load_vec<T, V>(dp + p * g.dy_pixel, d);
-        grad_z<V, SWISH>(u, d, add, rstd, gamma, beta, xhat, dz);
+    for_pixels<T, V>(w, r, rows, xp, g.x_pixel, dp, g.dy_pixel, [&](int64_t p, auto &raw, auto &up) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = rstd * (dz[j] * gamma[j] - ga - xhat[j] * gb);
-        store_vec<T, V>(op + p * g.channels, d);
-    }
+        for (int k = 0; k < kLoads; ++k) {
+            if (p + k * (int64_t)rows >= w.p1) continue;
+            float u[V], d[V], xhat[V], dz[V];
+            widen_vec<T, V>(raw[k], u);
+            widen_vec<T, V>(up[k], d);
+            grad_z<V, SWISH>(u, d, add, rstd, gamma, beta, xhat, dz);
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[j] = rstd * (dz[j] * gamma[j] - ga - xhat[j] * gb);
+            store_vec<T, V>(op + (p + k * (int64_t)rows) * g.channels, d);
+        }
+    });
 }
 
 // ---- one launch: a unit (sample, channel tile) held in the registers of one workgroup ---------------------------------
@@ -534,13 +568,6 @@ struct UnitArgs {
     float inv_q, inv_qg, inv_ng, inv_seats, eps, n, inv_n;   // n: values of a group
     const float *gamma, *beta, *shift;
 };
-// s / n with r near 1 / n: exact wherever the quotient is a float (a constant group's mean is its value)
-DEVI float over(float s, float n, float r)
-{
-    const float m = s * r;
-    return __builtin_fmaf(__builtin_fmaf(-m, n, s), r, m);
-}
-
 constexpr int kTileVecs = 64;   // vectors of a tile, unless one group (or the fewest whole groups that are whole vectors) is wider
 
 // V consecutive float32 from a 16-byte aligned place
@@ -932,7 +959,7 @@ int vec_of(const idm_group_norm_desc &d, bool backward, std::initializer_list<co
     return 1;
 }
 
-Geometry geometry_of(const idm_group_norm_desc &d, int v)
+Geometry geometry_of(const idm_group_norm_desc &d, bool backward, int v)
 {
     Geometry g = {};
     g.batch = d.batch; g.pixels = d.pixels;
@@ -941,19 +968,28 @@ Geometry geometry_of(const idm_group_norm_desc &d, int v)
     g.eps = d.eps;
     const int qg = g.gc / v;
     if (qg <= THREADS) {
-        g.gpt = std::min(g.groups, THREADS / qg);
+        // Few samples: tiles of 256 bytes, so that blocks come from the channels before they come from more chunks, which all have
+        // to be joined (1 x 4 096 x 512 float32, forward: 11 us, whole pixels 26).  Many: whole pixels, whose lines are read once.
+        const int wide = g.batch < 256 ? 256 / elem_bytes(d.dtype) / v : THREADS;
+        g.gpt = std::min(g.groups, std::max(1, wide / qg));
         g.tpg = 1;
+        g.ntile = (g.groups + g.gpt - 1) / g.gpt;
+        g.gpt = (g.groups + g.ntile - 1) / g.ntile;   // tiles of one width, nearly
         g.ntile = (g.groups + g.gpt - 1) / g.gpt;
     } else {
         g.gpt = 1;
         g.tpg = (qg + THREADS - 1) / THREADS;
         g.ntile = g.groups * g.tpg;
     }
-    // enough workgroups to fill the chip, none with less than a few vectors per thread
+    // Workgroups for the chip (backward some more: 1 024 x 784 x 90 fp16 180 us, with 1 024 of them 209; forward fewer: 8 x 65 536 x
+    // 32 bf16 24 us, with 1 536 of them 26), none with less than four vectors per thread, nor with more to join (12 bytes for a chunk
+    // and group) than it has to read itself; chunks of whole fours
     const int rows = std::max(1, THREADS / std::min(THREADS, g.gpt * qg));
-    const int64_t most = std::max<int64_t>(1, g.pixels / (4 * rows)), want = (2048 + g.batch * g.ntile - 1) / (g.batch * g.ntile);
-    int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, want, 1024}));
+    const int64_t most = std::max<int64_t>(1, g.pixels / (4 * rows)), tiles = g.batch * g.ntile, want = ((backward ? 1536 : 1024) + tiles - 1) / tiles;
+    const int64_t join = (int64_t)std::sqrt((double)g.pixels * g.gc * elem_bytes(d.dtype) / 12.0);
+    int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, want, join, 1024}));
     g.chunk = (g.pixels + n - 1) / n;
+    if (n > 1) g.chunk = (g.chunk + 4 * rows - 1) / (4 * rows) * (4 * rows);
     g.nchunk = (int)((g.pixels + g.chunk - 1) / g.chunk);
     return g;
 }
@@ -1065,7 +1101,7 @@ size_t workspace_floats(const idm_group_norm_desc &d, bool backward)
     if (!(unit && d.aligned))
         for (int v = 16 / elem_bytes(d.dtype); v >= 1; v >>= 1) {
             if ((d.channels / d.groups) % v) continue;
-            const Geometry g = geometry_of(d, v);
+            const Geometry g = geometry_of(d, backward, v);
             const size_t rows = (size_t)g.batch * g.nchunk;
             most = std::max(most, backward ? rows * (3 * g.channels + 2 * g.tpg * g.groups) : rows * g.tpg * g.groups * 3);
         }
@@ -1274,7 +1310,7 @@ int idm_group_norm_forward(int device, const idm_group_norm_desc *d, const void 
         });
     }
     const int v = vec_of(*d, false, {x_dev, y_dev});
-    Geometry g = geometry_of(*d, v);
+    Geometry g = geometry_of(*d, false, v);
     g.gamma = gamma_dev; g.beta = beta_dev; g.shift = shift_dev;
     return by_type(d->dtype, v, [&](auto t, auto w) {
         return forward_launch<decltype(t), decltype(w)::value>(*d, g, x_dev, y_dev, mean_dev, rstd_dev, (float *)workspace_dev, (hipStream_t)stream);
@@ -1307,7 +1343,7 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
         });
     }
     const int v = vec_of(*d, true, {dy_dev, x_dev, dx_dev});
-    Geometry g = geometry_of(*d, v);
+    Geometry g = geometry_of(*d, true, v);
     g.gamma = gamma_dev; g.beta = beta_dev; g.shift = shift_dev;
     return by_type(d->dtype, v, [&](auto t, auto w) {
         auto *f = d->activation == IDM_ACT_SWISH ? &backward_launch<decltype(t), decltype(w)::value, true>

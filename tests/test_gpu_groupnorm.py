@@ -137,6 +137,19 @@ def test_many_samples(shape, groups, dtype):
     verify(x, gamma, beta, shift, dy, groups, "swish" if n % 3 else "none")
 
 
+# few samples of many channels: tiles of a part of a pixel (the last one narrower, or one group wider than a tile), chunks whose last
+# rows are not full
+WIDE = [((2, 40, 41, 256), 32), ((1, 33, 31, 150), 15), ((3, 700, 520), 5), ((1, 64, 65, 512), 32), ((2, 50, 43, 264), 11), ((257, 5, 7, 300), 12)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,groups", WIDE)
+def test_few_samples_of_many_channels(shape, groups, dtype):
+    n = sum(shape) + groups
+    x, gamma, beta, shift, dy = inputs(shape, TYPES[dtype], n, groups, shift=["rows", "none", "one", "flat"][n % 4])
+    verify(x, gamma, beta, shift, dy, groups, "swish" if n % 3 else "none")
+
+
 @pytest.mark.parametrize("act", ["swish", "none"])
 @pytest.mark.parametrize("shift", ["rows", "one", "flat", "none"])
 def test_activation_and_shift(act, shift):
