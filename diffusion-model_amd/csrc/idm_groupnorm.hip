@@ -624,7 +624,8 @@ template <int V> DEVI Seat seat_of(const UnitArgs &g, int64_t pack, int tile)
     return s;
 }
 
-// Joins the pieces of each group of the block: `lanes` (a power of two) lanes take one group together.  load(entry of part, row) and
+// Joins the pieces of each group of the block: `lanes` (a power of two) lanes take one group together, as many as let all groups be
+// joined at once, four at least (2 x 100 x 24 in 3-channel groups, bf16, forward: 8.4 us; 15.4 with 64 lanes to each in turn).  load(entry of part, row) and
 // add work on a lane's running value, done(sub, group of the tile, value) runs on one lane of each group.  Pieces of a group are qg
 // consecutive ones of each row of `row` pieces.
 template <typename A, typename B, typename C> DEVI void fold_groups(const UnitArgs &g, int P, A &&first, B &&second, C &&done)
@@ -632,6 +633,7 @@ template <typename A, typename B, typename C> DEVI void fold_groups(const UnitAr
     const int entries = g.rows * g.qg, row = g.q * P, all = g.pack * g.ng;
     int lanes = 1;
     while (lanes < 64 && lanes < entries) lanes <<= 1;
+    while (lanes > 4 && lanes * all > (int)blockDim.x) lanes >>= 1;
     const int lane = threadIdx.x & (lanes - 1), step = (int)blockDim.x / lanes;
     for (int k0 = 0; k0 < all; k0 += step) {
         const int k = k0 + (int)threadIdx.x / lanes, sub = quotient(k, g.inv_ng), grp = k - sub * g.ng;
@@ -1053,14 +1055,16 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
     //  - the seats that hold values (rows are cut to whole wavefronts, the last vector of a thread may be empty);
     //  - the wavefronts at work: a block takes ceil(waves / 4) of a SIMD's places (forward 6 with 8 vectors, 4 with 16, 8 with 4; backward 2
     //    and 3, float32 3 and 4); 12 of them (backward 8) keep the memory busy; a block alone loads, computes and stores in turn;
-    //  - what a thread does besides its vectors (a fifth more with 4 of them; 16 leave fewer wavefronts);
-    //  - the parts of a pixel: blocks of one sample share its 128-byte lines, and parts that are no whole 32 bytes share sectors too;
+    //  - what a thread does besides its vectors (a fifth more with 4 of them, unless the joining of many small groups outweighs it; 16
+    //    leave fewer wavefronts);
+    //  - the parts of a pixel: blocks of one sample share its 128-byte lines, and parts that are no whole 32 bytes share sectors too
+    //    (of less weight in calls that do not fill the chip);
     //  - blocks for all compute units, and whole turns of the walkers.
     // Measured on three sets in turn, us, bf16: forward 1 024 x 784 x 96 in 12-channel groups, tiles of 48 / 96 / 192 bytes 83 / 77 / 83;
     // 1 024 x 784 x 64, tiles of 32 / 64 / 128 bytes 55 / 44 / 49; backward 1 024 x 196 x 192, tiles of 48 / 96 / 192 bytes 79 / 76 / 69,
     // 4 096 x 49 x 128, tiles of 32 / 64 / 128 bytes 62 / 47 / 45.
     const int64_t pixel = (int64_t)d.channels * e;
-    float best = 0.0f;
+    float best = 0.0f, worth = 0.0f;
     UnitPlan chosen = u;
     for (int i = 0; i < (backward ? 2 : 3); ++i)
         for (int tiles = 1; tiles <= std::min(units, 4096); ++tiles) {
@@ -1071,24 +1075,27 @@ bool plan_unit(const idm_group_norm_desc &d, bool backward, bool aligned, UnitPl
             const int64_t packs = (d.batch + u.pack - 1) / u.pack, part = (int64_t)u.q * 16;
             const float seats = (float)(u.rows * u.q * u.pack) / (float)u.threads * (float)d.pixels / (float)(u.rows * u.nv);
             const float shared = (float)std::min<int64_t>(128, pixel) / (float)part;
-            const float lines = std::max(0.5f, shared > 1.0f ? 1.0f - 0.06f * (shared - 1.0f) : 1.0f) * (part % 32 ? 0.85f : 1.0f);
+            const float lines = std::max(0.5f, shared > 1.0f ? 1.0f - 0.06f * (shared - 1.0f) : 1.0f) * (part < 32 ? 0.5f : part % 32 ? 0.85f : 1.0f);
+            const float fill = std::min(1.0f, (float)(packs * tiles) / 256.0f);
             for (int blocks = backward ? 1 : most; blocks <= most; ++blocks) {
-                float use = seats * lines * std::min(1.0f, (float)(blocks * waves) / (float)many) * (blocks > 1 + !backward ? 1.0f : blocks > 1 ? 0.97f : backward ? 0.9f : 0.85f) *
-                            (u.nv == 4 ? 0.8f : u.nv == 16 ? 0.95f : 1.0f);
-                use *= std::min(1.0f, (float)(packs * tiles) / 256.0f);
+                float use = seats * (1.0f - (1.0f - lines) * fill) * std::min(1.0f, (float)(blocks * waves) / (float)many) * (blocks > 1 + !backward ? 1.0f : blocks > 1 ? 0.97f : backward ? 0.9f : 0.85f) *
+                            (u.nv == 4 && (backward || u.pieces <= 2) ? 0.8f : u.nv == 16 ? 0.95f : 1.0f);
                 const int64_t want = std::max(1, 256 * blocks / tiles), turns = (packs + want - 1) / want, n = (packs + turns - 1) / turns;
                 if (backward) use *= (float)packs / (float)(turns * std::min(want, packs));
-                if (use > best) {
-                    best = use;
+                if (use * std::sqrt(fill) > best) {   // (few blocks: their own time counts, not the chip's)
+                    best = use * std::sqrt(fill);
+                    worth = use * fill;
                     chosen = u;
                     chosen.walkers = n;
                 }
             }
         }
     u = chosen;
-    // Few large units: the form that cuts a sample into chunks fills the chip (16 x 4 096 x 64 bf16, backward: 19.6 us against 23.6;
-    // 16 x 16 384 x 32 float32, forward: 26 against 41).  Small units are done before its second launch has begun.
-    return best > (backward ? 0.5f : 0.3f) || (best > 0.0f && d.pixels * u.q * 16 <= (backward ? 40960 : 65536));
+    // Few large units: the form that cuts a sample into chunks fills the chip (16 x 4 096 x 64 bf16, backward: 17.4 us against 23.6;
+    // 16 x 16 384 x 32 float32, forward: 23 against 41).  Small units are done before its second launch has begun (16 x 784 x 32
+    // float32, backward: 12.3 against 14.1), unless groups straddle vectors (23 x 784 x 48 in 3-channel groups, bf16: 18 against 14).
+    const int64_t bytes = d.pixels * u.q * 16;
+    return worth > (backward ? 0.5f : 0.3f) || (best > 0.0f && bytes <= (backward ? u.pieces == 1 ? 40960 : 16384 : u.q == 1 ? 65535 : 131072));
 }
 
 // What a call needs.  Unless the caller says that all pointers are aligned, the size query does not know which form and vector width
