@@ -137,33 +137,19 @@ SIGNATURES = {
     "idm_adamw_moments": (C.c_int, [C.c_int] + [C.c_void_p] * 6 + [C.c_int64, C.c_void_p]),
 }
 
-_lib = None
-_current_device = _raw_stream = _on_device = None      # of torch, bound by load()
-
-
-def call(entry, dev, args):
-    """``entry(device, *args, stream)`` on torch's current stream of ``dev``, with ``dev`` as the current device."""
-    index = dev.index
-    if _current_device() == index:
-        check(entry(index, *args, _raw_stream(index)))
-    else:
-        with _on_device(index):
-            check(entry(index, *args, _raw_stream(index)))
+_lib = _bound = None
 
 
 def load():
     """Load the shared library (once) and bind every exported symbol."""
-    global _lib, _current_device, _raw_stream, _on_device
+    global _lib
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise IdmError(f"{LIB_PATH} not found: build it with `make -C diffusion-model_amd/csrc` "
                            "(there is no CPU fallback)")
         # PyTorch bundles its own HIP runtime (same SONAME as /opt/rocm's).  Import it first so that
         # this library binds to the runtime that owns torch's device pointers and streams.
-        import torch
-        _current_device, _on_device = torch.cuda.current_device, torch.cuda.device
-        # the hipStream_t of a device's current stream; by torch's own short cut where it has one (0.1 us instead of 2)
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        import torch  # noqa: F401
         lib = C.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
@@ -173,6 +159,24 @@ def load():
             raise IdmError("libisingdiff.so ABI version mismatch")
         _lib = lib
     return _lib
+
+
+def host():
+    """The compiled host side of the training operators (``idm_host.cpp``), bound to the library (once)."""
+    global _bound
+    if _bound is None:
+        lib = load()
+        import torch
+        try:
+            from . import _host
+        except ImportError as e:
+            raise IdmError(f"isingdiff/_host.so cannot be loaded ({e}): build it with `make -C diffusion-model_amd/csrc`") from None
+        # the hipStream_t of a device's current stream; by torch's own short cut where it has one (0.1 us instead of 2)
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        names = ("group_norm_workspace", "group_norm_forward", "group_norm_backward", "adamw_step", "adamw_moments")
+        _host.bind(tuple(C.cast(getattr(lib, "idm_" + n), C.c_void_p).value for n in names), check, stream)
+        _bound = _host
+    return _bound
 
 
 def check(rc: int):

@@ -250,6 +250,21 @@ def test_captured_and_replayed_steps_go_on():
         assert int(state["step"]) == 5
 
 
+def test_gradients_that_are_views_and_parameters_without_versions():
+    from isingdiff import adamw_state, adamw_step
+    with torch.inference_mode():                      # (such tensors keep no version)
+        p = [torch.linspace(-1, 1, 12, device="cuda").reshape(3, 4), torch.ones(5, device="cuda")]
+    q = [t.clone() for t in p]
+    g = torch.randn(4, 3, device="cuda")
+    s, r = adamw_state(p), adamw_state(q)
+    adamw_step(p, [g.t(), torch._neg_view(q[1])], s)
+    adamw_step(q, [g.t().contiguous(), -q[1]], r)
+    assert all(torch.equal(a, b) for a, b in zip(p, q)) and all(torch.equal(s[k], r[k]) for k in s)
+    w, idle = torch.nn.Parameter(torch.ones(3, device="cuda")), torch.nn.Parameter(torch.ones(3, device="cuda"))
+    adamw_step([w, idle], [torch.ones(3, device="cuda"), None], adamw_state([w, idle]))
+    assert w._version == 1 and idle._version == 0     # only what changed
+
+
 def test_optimizer_class():
     from isingdiff import AdamW
     w = torch.nn.Parameter(torch.linspace(-1, 1, 600, device="cuda"))

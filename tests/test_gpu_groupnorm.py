@@ -209,6 +209,17 @@ def test_strided_vectors_of_parameters():
     assert torch.equal(a, group_norm_forward(x, wide[:, 0], wide[:, 1], 8, shift=two[..., 1])[0])
 
 
+def test_views_that_negate():
+    import isingdiff as I
+    x, gamma, beta, shift, dy = inputs((2, 6, 5, 16), torch.float32, 21, 4, shift="rows")
+    want = I.group_norm_forward(-x, gamma, beta, 4, shift=-shift)
+    got = I.group_norm_forward(torch._neg_view(x), gamma, beta, 4, shift=torch._neg_view(shift))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    want = I.group_norm_backward(-dy, -x, *want[1:], -gamma, beta, 4, shift=-shift)
+    got = I.group_norm_backward(torch._neg_view(dy), torch._neg_view(x), *got[1:], torch._neg_view(gamma), beta, 4, shift=torch._neg_view(shift))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_offsets_beyond_32_bits():
     """Two samples 2^31 + 64 elements apart in x and dy."""
     big = torch.empty((1 << 31) + 4096, dtype=torch.bfloat16, device="cuda")

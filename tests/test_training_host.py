@@ -29,6 +29,39 @@ def test_norm_refuses():
         group_norm_backward(x, x, torch.zeros(2, 8), torch.zeros(2, 8), one, one)
 
 
+def test_arguments_that_are_no_tensors():
+    x, p = torch.zeros(2, 4, 4, 16), [torch.zeros(300)]
+    s = adamw_state(p)
+    for gamma, beta, shift in (([1.0] * 16, None, None), (None, 1.0, None), (None, None, "shift")):
+        with pytest.raises(ValueError):
+            group_norm_forward(x, gamma, beta, shift=shift)
+    for groups in ("8", 8.0, None, 1 << 70):
+        with pytest.raises(ValueError):
+            group_norm_forward(x, None, None, groups)
+    for eps in (-1e-3, float("nan"), float("inf"), 1e39):
+        with pytest.raises(ValueError):
+            group_norm_forward(x, None, None, eps=eps)
+    with pytest.raises(TypeError):
+        group_norm_forward(x, None, None, eps="small")
+    for params, grads in ((p, [0.0]), ([None], [None]), ([p], [p]), (p, [torch.zeros(300).to_sparse()]), ([torch._neg_view(p[0])], p)):
+        with pytest.raises(ValueError):
+            adamw_step(params, grads, s)
+    with pytest.raises(TypeError):
+        adamw_step(p, 3, s)
+    with pytest.raises(ValueError):
+        adamw_step(p, p, s, betas=(0.9,))
+    with pytest.raises(KeyError):
+        adamw_step(p, p, {"m": s["m"], "v": s["v"]})
+    with pytest.raises(ValueError):
+        adamw_step(p, p, {**s, "v": None})
+    with pytest.raises(ValueError, match="CUDA"):
+        adamw_step(iter(p), (q for q in p), s, weight_decay=(0.1 for _ in p))
+
+
+def test_struct_layouts():
+    assert C.sizeof(_lib.GroupNormDesc) == 80 and C.sizeof(_lib.AdamWCfg) == 48
+
+
 def norm_desc(**over):
     f = dict(dtype=0, activation=1, batch=2, pixels=16, channels=16, groups=8, x_sample=256, x_pixel=16, dy_sample=256, dy_pixel=16,
              shift_sample=0, eps=1e-3, aligned=0)
