@@ -349,23 +349,24 @@ DEVI void grad_z(const float u[V], const float dy[V], const float add[V], float 
     }
 }
 
-// Sums over the rows of buf[rows][width]: done(c, sum) by one thread for each column.  Needs a barrier before and leaves with one.
-template <typename F> DEVI void sum_rows(float *buf, int rows, int width, F &&done)
+// Sums over the rows of buf, whose value (row, column) is at at(row, column): done(c, sum) by one thread for each column.  Needs a
+// barrier before and leaves with one.
+template <typename G, typename F> DEVI void sum_rows(float *buf, int rows, int width, G &&at, F &&done)
 {
     const int TH = (int)blockDim.x, split = TH / width < rows ? TH / width : rows;
     if (split > 1) {
         const int c = threadIdx.x % width, s = threadIdx.x / width;
         float t = 0.0f;
         if (s < split)
-            for (int k = s; k < rows; k += split) t += buf[k * width + c];
+            for (int k = s; k < rows; k += split) t += buf[at(k, c)];
         __syncthreads();
-        if (s < split) buf[s * width + c] = t;
+        if (s < split) buf[at(s, c)] = t;
         __syncthreads();
         rows = split;
     }
     for (int c = threadIdx.x; c < width; c += TH) {
         float t = 0.0f;
-        for (int k = 0; k < rows; ++k) t += buf[k * width + c];
+        for (int k = 0; k < rows; ++k) t += buf[at(k, c)];
         done(c, t);
     }
     __syncthreads();
@@ -419,7 +420,7 @@ __global__ __launch_bounds__(THREADS) void gn_grad_sums_kernel(Geometry g, const
 #pragma unroll
             for (int j = 0; j < V; ++j) sh[(r * q + cq) * V + j] = acc[i][j];
         __syncthreads();
-        sum_rows(sh, rows, w.width, [&](int c, float s) {
+        sum_rows(sh, rows, w.width, [&](int k, int c) { return k * w.width + c; }, [&](int c, float s) {
             sums[i * plane + row + w.c0 + c] = s;
             if (i < 2) by_channel[i][c] = (g.gamma ? g.gamma[w.c0 + c] : 1.0f) * s;
         });
@@ -794,28 +795,45 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
     const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ sums, float *__restrict__ dshift)
 {
     constexpr int V = vec16<T>, PS = V / P, E = sizeof(T);
+    constexpr bool AHEAD = E == 2 && NV == 4 && P <= 2;
     extern __shared__ float lds[];
     float *const total[2] = {lds, lds + blockDim.x * V}, *const buf = lds + 2 * blockDim.x * V;
     float2 *const part = (float2 *)buf, *const stat = (float2 *)(buf + blockDim.x * (V > 2 * P ? V : 2 * P));
     const int walker = blockIdx.z * gridDim.x + blockIdx.x;
     if (walker >= walkers) return;
+    // A thread's V values stand in quarters of a wavefront's 16-byte accesses, [V / 4][threads][4]: side by side they met in the same
+    // banks, a fifth of the kernel's time
+    const auto own = [&](int j) { return (j / 4 * (int)blockDim.x + (int)threadIdx.x) * 4 + j % 4; };
+    const auto at = [&](int row, int c) { return ((c % V) / 4 * (int)blockDim.x + row * g.q + c / V) * 4 + c % 4; };
     const int width = g.q * V, c0 = blockIdx.y * width;
     const int xpitch = (int)g.x_pixel * E, dpitch = (int)g.dy_pixel * E, opitch = g.channels * E;
 #pragma unroll
-    for (int j = 0; j < V; ++j) total[0][threadIdx.x * V + j] = total[1][threadIdx.x * V + j] = 0.0f;
-    for (int64_t pack = walker; pack * g.pack < g.batch; pack += walkers) {
-        const Seat s = seat_of<V>(g, pack, blockIdx.y);
-        const int64_t b0 = pack * g.pack;
-        u32x4 raw[NV], up[NV];
-        {
-            const auto xb = unit_buffer(x + b0 * g.x_sample + c0, kNowhere), db = unit_buffer(dy + b0 * g.dy_sample + c0, kNowhere);
-            const int xat = (int)(s.sub * g.x_sample) * E + s.r * xpitch + s.cq * 16, dat = (int)(s.sub * g.dy_sample) * E + s.r * dpitch + s.cq * 16;
+    for (int j = 0; j < V; ++j) total[0][own(j)] = total[1][own(j)] = 0.0f;
+    // Vector k of a pack (of one behind the last, nothing).  AHEAD: a vector's registers are free once it is used, so the next pack's is
+    // loaded into them there and then; memory works while the block computes, though a compute unit holds one such block only
+    // (1 024 x 14 x 14 x 192 bf16: 66 us, 70 without; 1 024 x 28 x 28 x 96: 157, 169).  With eight vectors, whose registers are short, and
+    // in float32, where two blocks take turns, it costs more than it gives (1 024 x 784 x 64 bf16: 100, 95; 512 x 784 x 64 float32: 98, 83).
+    Seat s = seat_of<V>(g, walker, blockIdx.y);
+    u32x4 raw[NV], up[NV];
+    const int xat = (int)(s.sub * g.x_sample) * E + s.r * xpitch + s.cq * 16, dat = (int)(s.sub * g.dy_sample) * E + s.r * dpitch + s.cq * 16;
+    const auto load_x = [&](const Seat &n, int64_t pack, int k) {
+        raw[k] = load16(unit_buffer(x + pack * g.pack * g.x_sample + c0, kNowhere), k < n.mine ? xat + k * g.rows * xpitch : kNowhere);
+    };
+    const auto load_dy = [&](const Seat &n, int64_t pack, int k) {
+        up[k] = load16(unit_buffer(dy + pack * g.pack * g.dy_sample + c0, kNowhere), k < n.mine ? dat + k * g.rows * dpitch : kNowhere);
+    };
+    const auto load_all = [&](int64_t pack) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                raw[k] = load16(xb, k < s.mine ? xat + k * g.rows * xpitch : kNowhere);
-                up[k] = load16(db, k < s.mine ? dat + k * g.rows * dpitch : kNowhere);
-            }
+        for (int k = 0; k < NV; ++k) {
+            load_x(s, pack, k);
+            load_dy(s, pack, k);
         }
+    };
+    if constexpr (AHEAD) load_all(walker);
+    for (int64_t pack = walker; pack * g.pack < g.batch; pack += walkers) {
+        const int64_t b0 = pack * g.pack;
+        const Seat next = seat_of<V>(g, pack + walkers, blockIdx.y);
+        if constexpr (!AHEAD) load_all(pack);
         // u = x + add (float32) or x (16 bits), xhat = u * rstd + off, z = u * a + sh.  The loop sums dz and dz * u; dz * xhat
         // follows from them.
         float add[V], off[V], rstd[P], a[V], sh[V];
@@ -840,24 +858,26 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
         for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (k >= s.mine) continue;
-            float u[V];
-            widen<T>(raw[k], u);
-            widen<T>(up[k], dz[k]);
-            if constexpr (E == 4)
+            if (k < s.mine) {
+                float u[V];
+                widen<T>(raw[k], u);
+                widen<T>(up[k], dz[k]);
+                if constexpr (E == 4)
 #pragma unroll
-                for (int j = 0; j < V; ++j) u[j] += add[j];
-            if (g.swish)
+                    for (int j = 0; j < V; ++j) u[j] += add[j];
+                if (g.swish)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float z = __builtin_fmaf(u[j], a[j], sh[j]), sg = sigmoid(z);
+                        dz[k][j] *= __builtin_fmaf(z * sg, 1.0f - sg, sg);
+                    }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float z = __builtin_fmaf(u[j], a[j], sh[j]), sg = sigmoid(z);
-                    dz[k][j] *= __builtin_fmaf(z * sg, 1.0f - sg, sg);
+                    s0[j] += dz[k][j];
+                    s1[j] = __builtin_fmaf(dz[k][j], u[j], s1[j]);
                 }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                s0[j] += dz[k][j];
-                s1[j] = __builtin_fmaf(dz[k][j], u[j], s1[j]);
             }
+            if constexpr (AHEAD) load_dy(next, pack + walkers, k);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = __builtin_fmaf(s1[j], rstd[j / PS], off[j] * s0[j]);
@@ -874,8 +894,8 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
         if (s.active)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                total[0][threadIdx.x * V + j] += s0[j];
-                total[1][threadIdx.x * V + j] += s1[j];
+                total[0][own(j)] += s0[j];
+                total[1][own(j)] += s1[j];
             }
         __syncthreads();
         fold_groups(
@@ -903,36 +923,39 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
         const int oat = (s.sub * g.pixels + s.r) * opitch + s.cq * 16;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (k >= s.mine) continue;
-            float u[V];
-            widen<T>(raw[k], u);
+            if (k < s.mine) {
+                float u[V];
+                widen<T>(raw[k], u);
 #pragma unroll
-            for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(dz[k][j], a[j], __builtin_fmaf(E == 2 ? u[j] : u[j] + add[j], cx[j / PS], c0v[j]));
-            if (dshift)
+                for (int j = 0; j < V; ++j) u[j] = __builtin_fmaf(dz[k][j], a[j], __builtin_fmaf(E == 2 ? u[j] : u[j] + add[j], cx[j / PS], c0v[j]));
+                if (dshift)
 #pragma unroll
-                for (int j = 0; j < V; ++j) s0[j] += u[j];
-            store16(ob, oat + k * g.rows * opitch, narrow<T>(u));
+                    for (int j = 0; j < V; ++j) s0[j] += u[j];
+                store16(ob, oat + k * g.rows * opitch, narrow<T>(u));
+            }
+            if constexpr (AHEAD) load_x(next, pack + walkers, k);
         }
         if (dshift) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) buf[threadIdx.x * V + j] = s0[j];
+            for (int j = 0; j < V; ++j) buf[own(j)] = s0[j];
             __syncthreads();
             if (g.pack == 1) {
-                sum_rows(buf, g.rows, width, [&](int k, float t) { dshift[b0 * g.channels + c0 + k] = t; });
+                sum_rows(buf, g.rows, width, at, [&](int k, float t) { dshift[b0 * g.channels + c0 + k] = t; });
             } else {   // few rows each
                 for (int i = threadIdx.x; i < g.pack * width; i += blockDim.x) {
                     const int sub = i / width, k = i - sub * width;
                     float t = 0.0f;
-                    for (int r = 0; r < g.rows; ++r) t += buf[(sub * g.rows + r) * width + k];
+                    for (int r = 0; r < g.rows; ++r) t += buf[at(sub * g.rows + r, k)];
                     if (b0 + sub < g.batch) dshift[(b0 + sub) * g.channels + c0 + k] = t;
                 }
                 __syncthreads();
             }
         }
+        s = next;
     }
     __syncthreads();
     for (int i = 0; i < 2; ++i)
-        sum_rows(total[i], g.rows * g.pack, width, [&](int k, float t) { sums[((int64_t)i * walkers + walker) * g.channels + c0 + k] = t; });
+        sum_rows(total[i], g.rows * g.pack, width, at, [&](int k, float t) { sums[((int64_t)i * walkers + walker) * g.channels + c0 + k] = t; });
 }
 
 // Grid: x 16 columns, y planes, z splits
