@@ -796,50 +796,67 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
 {
     constexpr int V = vec16<T>, PS = V / P, E = sizeof(T);
     constexpr bool AHEAD = E == 2 && NV == 4 && P <= 2;
-    extern __shared__ float lds[];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     float *const total[2] = {lds, lds + blockDim.x * V}, *const buf = lds + 2 * blockDim.x * V;
     float2 *const part = (float2 *)buf, *const stat = (float2 *)(buf + blockDim.x * (V > 2 * P ? V : 2 * P));
     const int walker = blockIdx.z * gridDim.x + blockIdx.x;
     if (walker >= walkers) return;
-    // A thread's V values stand in quarters of a wavefront's 16-byte accesses, [V / 4][threads][4]: side by side they met in the same
-    // banks, a fifth of the kernel's time
-    const auto own = [&](int j) { return (j / 4 * (int)blockDim.x + (int)threadIdx.x) * 4 + j % 4; };
+    // A thread's V values stand in 16-byte pieces, [V / 4][threads][4], so that a wavefront's accesses meet no bank twice.  Written one
+    // by one with eight vectors: registers that are neighbours are one demand too many there (512 x 784 x 64 float32: 85 us, 88).
+    const auto own = [&](float *b, const float v[V], bool add) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            float *const q = b + (j / 4 * (int)blockDim.x + (int)threadIdx.x) * 4;
+            if constexpr (NV == 4) {
+                const f32x4 w = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+                *(f32x4 *)q = add ? *(const f32x4 *)q + w : w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[i] = add ? q[i] + v[j + i] : v[j + i];
+            }
+        }
+    };
     const auto at = [&](int row, int c) { return ((c % V) / 4 * (int)blockDim.x + row * g.q + c / V) * 4 + c % 4; };
     const int width = g.q * V, c0 = blockIdx.y * width;
     const int xpitch = (int)g.x_pixel * E, dpitch = (int)g.dy_pixel * E, opitch = g.channels * E;
-#pragma unroll
-    for (int j = 0; j < V; ++j) total[0][own(j)] = total[1][own(j)] = 0.0f;
+    {
+        const float zero[V] = {};
+        own(total[0], zero, false);
+        own(total[1], zero, false);
+    }
     // Vector k of a pack (of one behind the last, nothing).  AHEAD: a vector's registers are free once it is used, so the next pack's is
     // loaded into them there and then; memory works while the block computes, though a compute unit holds one such block only
-    // (1 024 x 14 x 14 x 192 bf16: 66 us, 70 without; 1 024 x 28 x 28 x 96: 157, 169).  With eight vectors, whose registers are short, and
+    // (1 024 x 14 x 14 x 192 bf16: 64 us, 70 without; 1 024 x 28 x 28 x 96: 156, 169).  With eight vectors, whose registers are short, and
     // in float32, where two blocks take turns, it costs more than it gives (1 024 x 784 x 64 bf16: 100, 95; 512 x 784 x 64 float32: 98, 83).
-    Seat s = seat_of<V>(g, walker, blockIdx.y);
     u32x4 raw[NV], up[NV];
-    const int xat = (int)(s.sub * g.x_sample) * E + s.r * xpitch + s.cq * 16, dat = (int)(s.sub * g.dy_sample) * E + s.r * dpitch + s.cq * 16;
-    const auto load_x = [&](const Seat &n, int64_t pack, int k) {
-        raw[k] = load16(unit_buffer(x + pack * g.pack * g.x_sample + c0, kNowhere), k < n.mine ? xat + k * g.rows * xpitch : kNowhere);
-    };
-    const auto load_dy = [&](const Seat &n, int64_t pack, int k) {
-        up[k] = load16(unit_buffer(dy + pack * g.pack * g.dy_sample + c0, kNowhere), k < n.mine ? dat + k * g.rows * dpitch : kNowhere);
-    };
-    const auto load_all = [&](int64_t pack) {
+    const auto load = [&](const Seat &n, int64_t pack, int first, int last, bool of_x, bool of_dy) {
+        const auto xb = unit_buffer(x + pack * g.pack * g.x_sample + c0, kNowhere), db = unit_buffer(dy + pack * g.pack * g.dy_sample + c0, kNowhere);
+        const int xat = (int)(n.sub * g.x_sample) * E + n.r * xpitch + n.cq * 16, dat = (int)(n.sub * g.dy_sample) * E + n.r * dpitch + n.cq * 16;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            load_x(s, pack, k);
-            load_dy(s, pack, k);
+            if (k < first || k >= last) continue;
+            if (of_x) raw[k] = load16(xb, k < n.mine ? xat + k * g.rows * xpitch : kNowhere);
+            if (of_dy) up[k] = load16(db, k < n.mine ? dat + k * g.rows * dpitch : kNowhere);
         }
     };
-    if constexpr (AHEAD) load_all(walker);
+    Seat next;
+    if constexpr (AHEAD) {
+        next = seat_of<V>(g, walker, blockIdx.y);
+        load(next, walker, 0, NV, true, true);
+    }
     for (int64_t pack = walker; pack * g.pack < g.batch; pack += walkers) {
+        const Seat s = AHEAD ? next : seat_of<V>(g, pack, blockIdx.y);
         const int64_t b0 = pack * g.pack;
-        const Seat next = seat_of<V>(g, pack + walkers, blockIdx.y);
-        if constexpr (!AHEAD) load_all(pack);
+        if constexpr (AHEAD) next = seat_of<V>(g, pack + walkers, blockIdx.y);
+        else load(s, pack, 0, NV, true, true);
         // u = x + add (float32) or x (16 bits), xhat = u * rstd + off, z = u * a + sh.  The loop sums dz and dz * u; dz * xhat
         // follows from them.
         float add[V], off[V], rstd[P], a[V], sh[V];
         load_chan16<V>(g.shift && s.active ? g.shift + s.b * g.shift_sample : nullptr, s.c, 0.0f, add);
-        load_chan16<V>(s.active ? g.gamma : nullptr, s.c, 1.0f, a);
-        load_chan16<V>(s.active ? g.beta : nullptr, s.c, 0.0f, sh);
+        const float *gamma = g.gamma, *beta = g.beta;
+        asm volatile("" : "+s"(gamma), "+s"(beta));   // (read again for each pack: no registers to hold them)
+        load_chan16<V>(s.active ? gamma : nullptr, s.c, 1.0f, a);
+        load_chan16<V>(s.active ? beta : nullptr, s.c, 0.0f, sh);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int64_t at = s.active ? s.b * g.groups + blockIdx.y * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0;
@@ -877,7 +894,7 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
                     s1[j] = __builtin_fmaf(dz[k][j], u[j], s1[j]);
                 }
             }
-            if constexpr (AHEAD) load_dy(next, pack + walkers, k);
+            if constexpr (AHEAD) load(next, pack + walkers, k, k + 1, false, true);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = __builtin_fmaf(s1[j], rstd[j / PS], off[j] * s0[j]);
@@ -891,12 +908,10 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
             }
             part[threadIdx.x * P + i] = t;
         }
-        if (s.active)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                total[0][own(j)] += s0[j];
-                total[1][own(j)] += s1[j];
-            }
+        if (s.active) {
+            own(total[0], s0, true);
+            own(total[1], s1, true);
+        }
         __syncthreads();
         fold_groups(
             g, P,
@@ -933,11 +948,10 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
                     for (int j = 0; j < V; ++j) s0[j] += u[j];
                 store16(ob, oat + k * g.rows * opitch, narrow<T>(u));
             }
-            if constexpr (AHEAD) load_x(next, pack + walkers, k);
+            if constexpr (AHEAD) load(next, pack + walkers, k, k + 1, true, false);
         }
         if (dshift) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) buf[own(j)] = s0[j];
+            own(buf, s0, false);
             __syncthreads();
             if (g.pack == 1) {
                 sum_rows(buf, g.rows, width, at, [&](int k, float t) { dshift[b0 * g.channels + c0 + k] = t; });
@@ -951,7 +965,6 @@ __global__ __launch_bounds__(TH, NV == 8 ? sizeof(T) == 4 && P == 1 ? 3 : 2 : si
                 __syncthreads();
             }
         }
-        s = next;
     }
     __syncthreads();
     for (int i = 0; i < 2; ++i)
