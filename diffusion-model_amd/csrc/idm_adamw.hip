@@ -15,6 +15,14 @@
 // so that a second moment that changes by 0.1 % a step, a hundredth of a code, moves by one code in about a hundred steps, where
 // rounding to nearest would never move it.  A second moment above zero never gets code zero.  Entries that are not finite take the
 // largest code and leave their block's window to the others.
+//
+// Memory bounds it: parameter, gradient and moments are read once, parameter and moments written once, 28 bytes an entry with all of them
+// float32, 10 with 16-bit parameters and gradients and codes.  50 M entries float32: 268 us (5.2 TB/s; a large copy reaches 4.9, a sum of
+// two arrays 5.8); 100 M bf16 with codes: 215 us (4.7 TB/s; the codes' arithmetic is hidden to two thirds), their decoding 165 us (6.1 TB/s).
+// All tensors go in one launch for each 96: a workgroup takes 4 096 entries of one of them and finds it by bisection in a table that
+// travels with the arguments, so nothing is copied to the device first.  A kernel of one thread counts the step and prepares the bias
+// corrections (2 us; on the device, so that a captured step goes on counting).  66 small tensors: 9 us, which 4 096 entries a workgroup
+// keep to one turn of the chip.
 #include "../../include/isingdiff.h"
 #include "idm_internal.h"
 #include "idm_device.h"
@@ -25,6 +33,7 @@
 
 namespace {
 
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 constexpr int BLOCK = IDM_ADAMW_BLOCK;      // entries that share a window
 constexpr int CHUNK = 4096;                 // entries of one workgroup
 constexpr int TENSORS = 96;                 // tensors of one launch (their table travels in the kernel arguments, at most 4 KB)
@@ -107,7 +116,20 @@ DEVI float root_of(float v)
     return small ? r * 0x1p-32f : r;
 }
 
-template <typename PT, typename GT, bool EIGHT>
+// Moments are not looked at again before the next step.  Where a step's tensors exceed the 256 MB of cache (FAR), 32-bit ones pass
+// it by and leave it to parameters and gradients, which the passes before and after the step share.
+template <bool FAR, typename V> DEVI V take(const V *p)
+{
+    if constexpr (FAR) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool FAR, typename V> DEVI void put(V *p, V v)
+{
+    if constexpr (FAR) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
+template <typename PT, typename GT, bool EIGHT, bool FAR>
 __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__restrict__ coef, float b1, float c1, float b2, float c2,
                                                     float eps, void *__restrict__ m_all, void *__restrict__ v_all,
                                                     int16_t *__restrict__ m_base, int16_t *__restrict__ v_base)
@@ -135,15 +157,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
         load_entries<GT, N>(g, i, n, full, gv);
         const int64_t w = (at + i) / BLOCK;    // the block among the moments
         if constexpr (EIGHT) {
-            const uint2 cm = *(const uint2 *)((const uint8_t *)m_all + at + i), cv = *(const uint2 *)((const uint8_t *)v_all + at + i);
+            const u32x2 cm = take<FAR>((const u32x2 *)((const uint8_t *)m_all + at + i)), cv = take<FAR>((const u32x2 *)((const uint8_t *)v_all + at + i));
             const int bm = m_base[w], bv = v_base[w];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                m[j] = value_m((j < 4 ? cm.x : cm.y) >> 8 * (j & 3) & 255u, bm);
-                v[j] = value_v((j < 4 ? cv.x : cv.y) >> 8 * (j & 3) & 255u, bv);
+                m[j] = value_m(cm[j / 4] >> 8 * (j & 3) & 255u, bm);
+                v[j] = value_v(cv[j / 4] >> 8 * (j & 3) & 255u, bv);
             }
         } else {
-            const f32x4 mm = *(const f32x4 *)((const float *)m_all + at + i), vv = *(const f32x4 *)((const float *)v_all + at + i);
+            const f32x4 mm = take<FAR>((const f32x4 *)((const float *)m_all + at + i)), vv = take<FAR>((const f32x4 *)((const float *)v_all + at + i));
 #pragma unroll
             for (int j = 0; j < N; ++j) { m[j] = mm[j]; v[j] = vv[j]; }
         }
@@ -189,15 +211,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
                 cm[j >> 2] |= ((uint32_t)a | (__float_as_uint(m[j]) >> 24 & 128u)) << 8 * (j & 3);
                 cv[j >> 2] |= (uint32_t)b << 8 * (j & 3);
             }
-            *(uint2 *)((uint8_t *)m_all + at + i) = uint2{cm[0], cm[1]};
-            *(uint2 *)((uint8_t *)v_all + at + i) = uint2{cv[0], cv[1]};
+            put<FAR>((u32x2 *)((uint8_t *)m_all + at + i), u32x2{cm[0], cm[1]});
+            put<FAR>((u32x2 *)((uint8_t *)v_all + at + i), u32x2{cv[0], cv[1]});
             if ((threadIdx.x & (LANES - 1)) == 0) {
                 m_base[w] = (int16_t)bm;
                 v_base[w] = (int16_t)bv;
             }
         } else {
-            *(f32x4 *)((float *)m_all + at + i) = f32x4{m[0], m[1], m[2], m[3]};
-            *(f32x4 *)((float *)v_all + at + i) = f32x4{v[0], v[1], v[2], v[3]};
+            put<FAR>((f32x4 *)((float *)m_all + at + i), f32x4{m[0], m[1], m[2], m[3]});
+            put<FAR>((f32x4 *)((float *)v_all + at + i), f32x4{v[0], v[1], v[2], v[3]});
         }
     }
 }
@@ -280,6 +302,8 @@ try {
     Coef *coef = (Coef *)scratch_dev;
     hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, s, step_dev, cfg->lr, cfg->beta1, cfg->beta2, coef);
     const float b1 = (float)cfg->beta1, c1 = (float)(1 - cfg->beta1), b2 = (float)cfg->beta2, c2 = (float)(1 - cfg->beta2);
+    // (50 M float32: 267 us, 278 through the cache; 33 M: 140 and 190; below the limit it costs up to a twentieth, and codes gain nothing)
+    const bool far = !eight && total * (int64_t)(pb + gb + 8) > (int64_t)1 << 28;
     int64_t at = 0;
     Table tab;
     int64_t chunks = 0;
@@ -290,7 +314,7 @@ try {
         auto go = [&](auto p, auto g) {
             using PT = decltype(p);
             using GT = decltype(g);
-            auto kernel = eight ? &adamw_kernel<PT, GT, true> : &adamw_kernel<PT, GT, false>;
+            auto kernel = eight ? &adamw_kernel<PT, GT, true, false> : far ? &adamw_kernel<PT, GT, false, true> : &adamw_kernel<PT, GT, false, false>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(256), 0, s, tab, (const Coef *)coef, b1, c1, b2, c2, (float)cfg->eps, m_dev,
                                v_dev, m_base_dev, v_base_dev);
             return IDM_OK;

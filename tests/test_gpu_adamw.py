@@ -250,6 +250,23 @@ def test_captured_and_replayed_steps_go_on():
         assert int(state["step"]) == 5
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_moments_that_pass_the_cache_by(kind):
+    """A large step is the same, bit for bit, as steps over its parts, which stay in the cache."""
+    from isingdiff import adamw_state, adamw_step
+    n, part = (23 << 20) + 100, 8 << 20
+    gen = torch.Generator("cuda").manual_seed(5)
+    p, g = (torch.randn(n, device="cuda", generator=gen).to(TYPES[kind]) for _ in range(2))
+    parts = [t.clone() for t in p.split(part)]
+    state, states = adamw_state([p]), [adamw_state([t]) for t in parts]
+    for k in range(3):
+        adamw_step([p], [g], state)
+        for t, u, s in zip(parts, g.split(part), states):
+            adamw_step([t], [u], s)
+        g.mul_(-0.5)
+    assert torch.equal(p, torch.cat(parts)) and all(torch.equal(state[k], torch.cat([s[k] for s in states])) for k in "mv")
+
+
 def test_gradients_that_are_views_and_parameters_without_versions():
     from isingdiff import adamw_state, adamw_step
     with torch.inference_mode():                      # (such tensors keep no version)
