@@ -295,6 +295,14 @@ try {
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
         if (spans[i].first < spans[i - 1].second) return idm_set_error(IDM_ERR_INVALID, "adamw: two parameters share memory");
+    for (int64_t i = 0; i < n_tensors; ++i) {   // workgroups read gradients while others write parameters
+        if (!sizes[i] || !grads_dev[i]) continue;
+        const uintptr_t lo = (uintptr_t)grads_dev[i], hi = lo + (size_t)sizes[i] * gb;
+        auto after = std::lower_bound(spans.begin(), spans.end(), std::make_pair(hi, (uintptr_t)0));   // the first one from hi on
+        for (; after != spans.begin() && (after - 1)->second > lo; --after)
+            if ((after - 1)->first != lo || params_dev[i] != grads_dev[i] || pb != gb)
+                return idm_set_error(IDM_ERR_INVALID, "adamw: a gradient shares memory with a parameter");
+    }
     if (total && (!m_dev || !v_dev || (eight && (!m_base_dev || !v_base_dev)))) return idm_set_error(IDM_ERR_INVALID, "adamw: null moments");
     if ((uintptr_t)m_dev % 16 || (uintptr_t)v_dev % 16) return idm_set_error(IDM_ERR_INVALID, "adamw: moments must be aligned to 16 bytes");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "adamw: no such device");

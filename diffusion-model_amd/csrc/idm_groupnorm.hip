@@ -1246,7 +1246,7 @@ int check_desc(const idm_group_norm_desc *d, bool backward)
     if (d->batch < 0 || d->pixels < 0 || d->channels <= 0 || d->groups <= 0 || d->channels % d->groups)
         return idm_set_error(IDM_ERR_INVALID, "group norm: channels must be a positive multiple of groups, batch and pixels not negative");
     if (!(d->eps >= 0.0f) || std::isinf(d->eps)) return idm_set_error(IDM_ERR_INVALID, "group norm: eps must be finite and not negative");
-    if (d->channels > (1 << 20) || d->pixels > ((int64_t)1 << 40) || d->batch > ((int64_t)1 << 31))
+    if (d->channels > (1 << 20) || d->pixels > ((int64_t)1 << 40) || d->batch > ((int64_t)1 << 30))
         return idm_set_error(IDM_ERR_INVALID, "group norm: more than 2^20 channels, 2^40 pixels or 2^30 samples");
     if (d->x_pixel < d->channels || (backward && d->dy_pixel < d->channels))
         return idm_set_error(IDM_ERR_INVALID, "group norm: a pixel's stride is less than its channels");

@@ -331,6 +331,7 @@ State state_of(PyObject *dict, int64_t total, const c10::Device *dev)
             refuse(std::string("state['") + kKeys[k] + "'] must be " + std::to_string(n) + " dense " + c10::toString(want) + " values on " +
                    on.str() + ": make it with adamw_state for these parameters");
     }
+    if (total && s.at(M) == s.at(V)) refuse("state['m'] and state['v'] are the same memory");
     return s;
 }
 

@@ -268,6 +268,8 @@ class BitflipTrainer:
     def logits(self, X, t):
         """(B,H,W) float32: the flip probabilities before the sigmoid, with gradients for ``params``."""
         torch, p = self.torch, self.params
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("a training step checks its inputs on the host: it cannot be captured into a graph")
         dev = self.emb.device
         X, t = torch.as_tensor(X).to(dev), torch.as_tensor(t)
         if X.dim() != 3 or X.shape[1] % 4 or X.shape[2] % 4 or 0 in X.shape:

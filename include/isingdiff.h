@@ -387,7 +387,8 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
 /* One AdamW step over n_tensors tensors: t = *step_dev + 1 (written back), and per entry
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * params / grads / sizes / weight_decay: host arrays of n_tensors device pointers, entry counts and decays; a NULL gradient leaves
- * its tensor and moments as they are.  Gradients and parameters are dense; parameters must not share memory.
+ * its tensor and moments as they are.  Gradients and parameters are dense; parameters must not share memory,
+ * nor a gradient with a parameter (but for its own, entry by entry).
  * Moments: tensor i's begin at the sum of the sizes before it, each rounded up to IDM_ADAMW_BLOCK entries; `moments` is that sum
  * over all tensors.  moment_bits 32: m_dev, v_dev float32, bases unused.  8: bytes, with one int16 base per block of
  * IDM_ADAMW_BLOCK entries; code c > 0 stands for the float32 with bits (c + base) << 20 (m: bit 7 is the sign), rounded with a

@@ -100,3 +100,14 @@ def test_refusals():
                  (X, t * 0 + 100, flips), (X, t * 0 - 1, flips)):
         with pytest.raises(ValueError):
             tr.step(*args)
+
+
+def test_a_step_is_not_captured():
+    from isingdiff import bitflip
+    trainer = bitflip.BitflipTrainer(bitflip.synthetic_weights(0), time_step=10)
+    X, t = torch.zeros(2, 4, 4, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            trainer.step(X, t, X)
+    assert bool(torch.isfinite(trainer.step(X, t, X)))

@@ -209,6 +209,36 @@ def test_strided_vectors_of_parameters():
     assert torch.equal(a, group_norm_forward(x, wide[:, 0], wide[:, 1], 8, shift=two[..., 1])[0])
 
 
+def test_subnormal_halves():
+    """Values below 2^-14, which fp16 holds with fewer bits, have a mean and a deviation like others."""
+    import isingdiff as I
+    x, gamma, beta, _, _ = inputs((130, 5, 8, 32), torch.float16, 22, 4)
+    x = (x.float() * 2.0 ** -18).half()
+    _, mean, rstd = I.group_norm_forward(x, gamma, beta, 4, eps=1e-18, activation="none")
+    g = x.cpu().double().reshape(130, 40, 4, 8)
+    m, v = g.mean((1, 3)), g.var((1, 3), correction=0)
+    check("mean", mean, m, 64 * E * g.abs().mean((1, 3)))
+    check("rstd", rstd, (v + 1e-18).rsqrt(), 64 * E * (v + 1e-18).rsqrt() * (1 + g.pow(2).mean((1, 3)) / v))
+
+
+@pytest.mark.parametrize("samples", [4194304, 530000])
+def test_more_samples_than_one_grid(samples):
+    """Many copies of a few samples give many copies of their results."""
+    import isingdiff as I
+    pixels = 520 if samples == 530000 else 2
+    x, gamma, beta, _, dy = inputs((1000, pixels, 8), torch.float16, 23, 2)
+    n = samples // 1000
+    many = lambda t: t.repeat(n, 1, 1)  # noqa: E731
+    y, mean, rstd = I.group_norm_forward(many(x), gamma, beta, 2)
+    for t in (y, mean, rstd):
+        t = t.view(n, -1)
+        assert bool((t == t[:1]).all())
+    dx = I.group_norm_backward(many(dy), many(x), mean, rstd, gamma, beta, 2)[0].view(n, -1)
+    assert bool((dx == dx[:1]).all()) and bool(torch.isfinite(dx).all())
+    w = I.group_norm_forward(x, gamma, beta, 2)[0]
+    assert float((y[:1000].float() - w.float()).abs().max()) <= 2.0 ** -10 * float(w.float().abs().max())
+
+
 def test_views_that_negate():
     import isingdiff as I
     x, gamma, beta, shift, dy = inputs((2, 6, 5, 16), torch.float32, 21, 4, shift="rows")

@@ -52,8 +52,9 @@ def test_arguments_that_are_no_tensors():
         adamw_step(p, p, s, betas=(0.9,))
     with pytest.raises(KeyError):
         adamw_step(p, p, {"m": s["m"], "v": s["v"]})
-    with pytest.raises(ValueError):
-        adamw_step(p, p, {**s, "v": None})
+    for bad in ({**s, "v": None}, {**s, "v": s["m"]}):
+        with pytest.raises(ValueError):
+            adamw_step(p, p, bad)
     with pytest.raises(ValueError, match="CUDA"):
         adamw_step(iter(p), (q for q in p), s, weight_decay=(0.1 for _ in p))
 
@@ -74,7 +75,7 @@ def test_norm_entry_points_refuse():
     assert lib.idm_group_norm_workspace(C.byref(norm_desc()), 0, C.byref(size)) == 0 and size.value > 0
     for bad in (dict(dtype=3), dict(activation=2), dict(batch=-1), dict(pixels=-1), dict(channels=0), dict(groups=0), dict(groups=5),
                 dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(x_pixel=15), dict(x_sample=-1), dict(shift_sample=-1),
-                dict(channels=1 << 21, groups=1, x_pixel=1 << 21), dict(batch=1 << 32)):
+                dict(channels=1 << 21, groups=1, x_pixel=1 << 21), dict(batch=1 << 32), dict(batch=(1 << 30) + 1)):
         d = norm_desc(**bad)
         assert lib.idm_group_norm_workspace(C.byref(d), 0, C.byref(size)) == -1, bad
         assert lib.idm_group_norm_forward(0, C.byref(d), *[16] * 8, 1 << 30, None) == -1, bad
@@ -163,7 +164,8 @@ def test_adamw_entry_points_refuse():
     for bad in (dict(param_dtype=3), dict(grad_dtype=-1), dict(moment_bits=16), dict(lr=-1.0), dict(lr=float("inf")), dict(beta1=1.0),
                 dict(beta2=float("nan")), dict(eps=-1.0), dict(n=-1), dict(sizes=(300, -1)), dict(sizes=(300, 1 << 41)), dict(moments=512),
                 dict(moments=0), dict(params=(1 << 20, None)), dict(params=(1 << 20, (1 << 21) + 2)), dict(grads=(1 << 22, (1 << 23) + 1)),
-                dict(params=(1 << 20, 1 << 20)), dict(params=(1 << 20, (1 << 20) + 1196)), dict(decay=(0.0, -1.0)),
+                dict(params=(1 << 20, 1 << 20)), dict(params=(1 << 20, (1 << 20) + 1196)), dict(grads=(1 << 22, 1 << 20)), dict(grads=((1 << 20) + 4, 1 << 23)),
+                dict(grads=((1 << 21) - 1196, 1 << 23)), dict(grads=(1 << 20, 1 << 23), grad_dtype=1), dict(decay=(0.0, -1.0)),
                 dict(decay=(0.0, float("nan"))), dict(m=None), dict(v=8200), dict(base=(None, 32768)), dict(step=None), dict(scratch=None)):
         assert adamw_call(**bad) == -1, bad
         assert b"adamw" in _lib.load().idm_last_error()
