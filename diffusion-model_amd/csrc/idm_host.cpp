@@ -12,8 +12,11 @@
 #include <ATen/ops/full.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cmath>
@@ -294,6 +297,23 @@ PyObject *layout_py(PyObject *, PyObject *t)
     });
 }
 
+// Whether a backward pass that is captured on the current stream would add into the gradient of one of these on another stream: a leaf
+// adds on the stream of the first graph that it was part of, as long as one of those is alive.  (Such a capture ends the process.)
+PyObject *adds_elsewhere(PyObject *, PyObject *const *arg, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject * {
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!THPVariable_Check(arg[i])) continue;
+            const at::Tensor &t = THPVariable_Unpack(arg[i]);
+            if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
+            const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+            const auto at = node ? node->stream() : std::nullopt;
+            if (at && *at != c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device())) Py_RETURN_TRUE;
+        }
+        Py_RETURN_FALSE;
+    });
+}
+
 // ---- AdamW ---------------------------------------------------------------------------------------------------------------------
 
 constexpr int64_t BLOCK = IDM_ADAMW_BLOCK;
@@ -481,6 +501,7 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"group_norm_forward", (PyCFunction)(void *)with<group_norm_forward, 7>, METH_FASTCALL, nullptr},
     {"group_norm_backward", (PyCFunction)(void *)with<group_norm_backward, 9>, METH_FASTCALL, nullptr},
+    {"adds_elsewhere", (PyCFunction)(void *)adds_elsewhere, METH_FASTCALL, nullptr},
     {"layout", layout_py, METH_O, nullptr},
     {"adamw_step", (PyCFunction)(void *)with<adamw_step, 7>, METH_FASTCALL, nullptr},
     {"adamw_moments", adamw_moments, METH_O, nullptr},

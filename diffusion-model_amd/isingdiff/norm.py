@@ -51,6 +51,10 @@ class _GroupNorm(torch.autograd.Function):
 
 def group_norm(x, gamma=None, beta=None, groups: int = 8, *, shift=None, eps: float = 1e-3, activation: str = "swish"):
     """``act(GroupNorm(x + shift))`` with gradients for x, gamma, beta and shift (once differentiable).  gamma, beta and shift may
-    be of any floating type here; they are computed with in float32."""
+    be of any floating type here; they are computed with in float32.  May be captured into a HIP graph with its backward pass, but not
+    while a graph of an eager pass over the same leaves is alive."""
+    if (isinstance(x, torch.Tensor) and x.is_cuda and torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled()
+            and host().adds_elsewhere(x, gamma, beta, shift)):
+        raise ValueError("a graph of an eager pass over these leaves is alive: drop it (its loss) before a backward pass is captured")
     up = lambda t: None if t is None else t.float()  # noqa: E731
     return _GroupNorm.apply(x, up(gamma), up(beta), up(shift), groups, eps, activation)

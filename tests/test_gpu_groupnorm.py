@@ -418,6 +418,32 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(out, want)), k
 
 
+def test_a_backward_pass_is_captured_once_eager_graphs_are_gone():
+    from isingdiff import group_norm, group_norm_backward, group_norm_forward
+    x, gamma, beta, shift, dy = inputs((9, 6, 5, 32), torch.float32, 31, 8)
+    leaves = [t.requires_grad_() for t in (x, gamma, beta, shift)]
+    eager = group_norm(x, gamma, beta, 8, shift=shift)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            group_norm(x, gamma, beta, 8, shift=shift)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = group_norm(x, gamma, beta, 8, shift=shift)
+        y.backward(dy)
+    for k in range(3):
+        with torch.no_grad():
+            for t, new in zip(leaves + [dy], inputs((9, 6, 5, 32), torch.float32, 40 + k, 8)):
+                t.copy_(new)
+        graph.replay()
+        with torch.no_grad():
+            want, mean, rstd = group_norm_forward(x, gamma, beta, 8, shift=shift)
+            grads = group_norm_backward(dy, x, mean, rstd, gamma, beta, 8, shift=shift)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and all(torch.equal(t.grad, w) for t, w in zip(leaves, grads)), k
+
+
 def test_half_overflow_is_infinite():
     from isingdiff import group_norm_forward
     x, _, _, _, _ = inputs((1, 4, 4, 8), torch.float16, 2, 1)
