@@ -20,9 +20,8 @@
 // float32, 10 with 16-bit parameters and gradients and codes.  50 M entries float32: 268 us (5.2 TB/s; a large copy reaches 4.9, a sum of
 // two arrays 5.8); 100 M bf16 with codes: 215 us (4.7 TB/s; the codes' arithmetic is hidden to two thirds), their decoding 165 us (6.1 TB/s).
 // All tensors go in one launch for each 96: a workgroup takes 4 096 entries of one of them and finds it by bisection in a table that
-// travels with the arguments, so nothing is copied to the device first.  A kernel of one thread counts the step and prepares the bias
-// corrections (2 us; on the device, so that a captured step goes on counting).  66 small tensors: 9 us, which 4 096 entries a workgroup
-// keep to one turn of the chip.
+// travels with the arguments, so nothing is copied to the device first.  The step is counted and the bias corrected on the device, so
+// that a captured step goes on counting: by a kernel of one thread before a large step (2 us and a launch), within a small one.
 #include "../../include/isingdiff.h"
 #include "idm_internal.h"
 #include "idm_device.h"
@@ -54,13 +53,27 @@ struct Coef {
     uint32_t t, unused;
 };
 
-__global__ void adamw_begin_kernel(int64_t *step, double lr, double b1, double b2, Coef *c)
+// Where the step count stands, and what the coefficients of a step follow from (log1, log2: binary logarithms of the betas)
+struct Clock {
+    int64_t *step;
+    double lr, log1, log2;
+};
+
+DEVI Coef coef_of(int64_t t, const Clock &c)
 {
-    const int64_t t = *step + 1;
-    *step = t;
-    c->size = (float)(lr / (1.0 - pow(b1, (double)t)));
-    c->root = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
-    c->t = (uint32_t)t;
+    return {(float)(c.lr / (1.0 - exp2((double)t * c.log1))), (float)(1.0 / sqrt(1.0 - exp2((double)t * c.log2))), (uint32_t)t, 0};
+}
+
+// A step of one launch of at most kOnce workgroups counts itself: they all read the count, and each adds one to the bits above it when
+// // it has done so; the last of them moves the count on and clears those bits.  Larger steps begin with a kernel of one thread: the
+// additions go one after the other (one workgroup 3.8 us instead of 4.8 and 3 us less of host, 198 of them 8.2 and 8.5, 960 27 and 21).
+constexpr int kOnce = 256, kCountBits = 53;
+
+__global__ void adamw_begin_kernel(Clock clock, Coef *c)
+{
+    const int64_t t = *clock.step + 1;
+    *clock.step = t;
+    *c = coef_of(t, clock);
 }
 
 DEVI float value_m(uint32_t code, int base)
@@ -130,7 +143,7 @@ template <bool FAR, typename V> DEVI void put(V *p, V v)
 }
 
 template <typename PT, typename GT, bool EIGHT, bool FAR>
-__global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__restrict__ coef, float b1, float c1, float b2, float c2,
+__global__ __launch_bounds__(256) void adamw_kernel(Table tab, Clock clock, const Coef *__restrict__ coef, float b1, float c1, float b2, float c2,
                                                     float eps, void *__restrict__ m_all, void *__restrict__ v_all,
                                                     int16_t *__restrict__ m_base, int16_t *__restrict__ v_base)
 {
@@ -146,8 +159,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
     const GT *g = (const GT *)tab.g[k];
     const int64_t n = tab.n[k], at = (int64_t)tab.at[k] * BLOCK, i0 = (int64_t)(chunk - tab.first[k]) * CHUNK;
     const bool aligned = ((uintptr_t)p % (N * sizeof(PT)) | (uintptr_t)g % (N * sizeof(GT))) == 0;
-    const float keep = tab.keep[k], size = coef->size, root = coef->root;
-    const uint32_t t = coef->t;
+    const int64_t steps = coef ? 0 : (*clock.step & (((int64_t)1 << kCountBits) - 1)) + 1;
+    const Coef now = coef ? *coef : coef_of(steps, clock);
+    const float keep = tab.keep[k], size = now.size, root = now.root;
+    const uint32_t t = now.t;
 #pragma unroll 2
     for (int64_t i = i0 + threadIdx.x * N; i < i0 + CHUNK; i += 256 * N) {
         if (i / BLOCK * BLOCK >= n) break;     // (the same for all lanes of a block)
@@ -222,6 +237,14 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, const Coef *__res
             put<FAR>((f32x4 *)((float *)v_all + at + i), f32x4{v[0], v[1], v[2], v[3]});
         }
     }
+    if (!coef) {
+        __syncthreads();   // all wavefronts have read the count
+        if (threadIdx.x == 0) {
+            typedef unsigned long long word;
+            const word before = __hip_atomic_fetch_add((word *)clock.step, (word)1 << kCountBits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (before >> kCountBits == gridDim.x - 1) __hip_atomic_store((word *)clock.step, (word)steps, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
 }
 
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t *__restrict__ m, const uint8_t *__restrict__ v,
@@ -277,7 +300,7 @@ try {
     if (!(cfg->lr >= 0) || std::isinf(cfg->lr) || !(cfg->beta1 >= 0 && cfg->beta1 < 1) || !(cfg->beta2 >= 0 && cfg->beta2 < 1) ||
         !(cfg->eps >= 0) || std::isinf(cfg->eps))
         return idm_set_error(IDM_ERR_INVALID, "adamw: lr and eps must be finite and not negative, the betas in [0, 1)");
-    int64_t total = 0;
+    int64_t total = 0, work = 0;                // entries of the moments, workgroups
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     const size_t pb = cfg->param_dtype == IDM_DT_F32 ? 4 : 2, gb = cfg->grad_dtype == IDM_DT_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {
@@ -288,6 +311,7 @@ try {
         if (!sizes[i] || !grads_dev[i]) continue;
         if (!params_dev[i]) return idm_set_error(IDM_ERR_INVALID, "adamw: null parameter");
         if ((uintptr_t)params_dev[i] % pb || (uintptr_t)grads_dev[i] % gb) return idm_set_error(IDM_ERR_INVALID, "adamw: misaligned tensor");
+        work += (sizes[i] + CHUNK - 1) / CHUNK;
         spans.push_back({(uintptr_t)params_dev[i], (uintptr_t)params_dev[i] + (size_t)sizes[i] * pb});
     }
     if (total / BLOCK > 0xffffffff) return idm_set_error(IDM_ERR_INVALID, "adamw: more than 2^40 entries");
@@ -307,8 +331,9 @@ try {
     if ((uintptr_t)m_dev % 16 || (uintptr_t)v_dev % 16) return idm_set_error(IDM_ERR_INVALID, "adamw: moments must be aligned to 16 bytes");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "adamw: no such device");
     hipStream_t s = (hipStream_t)stream;
-    Coef *coef = (Coef *)scratch_dev;
-    hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, s, step_dev, cfg->lr, cfg->beta1, cfg->beta2, coef);
+    const Clock clock = {step_dev, cfg->lr, std::log2(cfg->beta1), std::log2(cfg->beta2)};
+    Coef *coef = work && spans.size() <= (size_t)TENSORS && work <= kOnce ? nullptr : (Coef *)scratch_dev;
+    if (coef) hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, s, clock, coef);
     const float b1 = (float)cfg->beta1, c1 = (float)(1 - cfg->beta1), b2 = (float)cfg->beta2, c2 = (float)(1 - cfg->beta2);
     // (50 M float32: 267 us, 278 through the cache; 33 M: 140 and 190; below the limit it costs up to a twentieth, and codes gain nothing)
     const bool far = !eight && total * (int64_t)(pb + gb + 8) > (int64_t)1 << 28;
@@ -323,7 +348,7 @@ try {
             using PT = decltype(p);
             using GT = decltype(g);
             auto kernel = eight ? &adamw_kernel<PT, GT, true, false> : far ? &adamw_kernel<PT, GT, false, true> : &adamw_kernel<PT, GT, false, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(256), 0, s, tab, (const Coef *)coef, b1, c1, b2, c2, (float)cfg->eps, m_dev,
+            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(256), 0, s, tab, clock, (const Coef *)coef, b1, c1, b2, c2, (float)cfg->eps, m_dev,
                                v_dev, m_base_dev, v_base_dev);
             return IDM_OK;
         };

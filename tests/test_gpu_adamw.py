@@ -267,6 +267,24 @@ def test_moments_that_pass_the_cache_by(kind):
     assert torch.equal(p, torch.cat(parts)) and all(torch.equal(state[k], torch.cat([s[k] for s in states])) for k in "mv")
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [256 * 4096, 256 * 4096 + 1])
+def test_both_ways_to_count_a_step(n, bits):
+    """256 workgroups count the step among themselves, more have it counted before: from equal states, equal steps."""
+    from isingdiff import adamw_state, adamw_step
+    gen = torch.Generator("cuda").manual_seed(6)
+    p, g = (torch.randn(n, device="cuda", generator=gen) for _ in range(2))
+    q, idle = p.clone(), torch.zeros(256 * 4096, device="cuda")      # the second tensor makes it a large step
+    s, r = adamw_state([p], bits), adamw_state([q, idle], bits)
+    for k in range(5):
+        adamw_step([p], [g], s, lr=0.1)
+        adamw_step([q, idle], [g, idle.clone()], r, lr=0.1)
+        assert int(s["step"]) == int(r["step"]) == k + 1
+        g.mul_(-0.8)
+    m = s["m"].numel()
+    assert torch.equal(p, q) and torch.equal(s["m"], r["m"][:m]) and torch.equal(s["v"], r["v"][:m])
+
+
 def test_gradients_that_are_views_and_parameters_without_versions():
     from isingdiff import adamw_state, adamw_step
     with torch.inference_mode():                      # (such tensors keep no version)
