@@ -294,6 +294,7 @@ int idm_adamw_step(int device, const idm_adamw_cfg *cfg, int64_t n_tensors, void
 try {
     if (!cfg || n_tensors < 0 || (n_tensors > 0 && (!params_dev || !grads_dev || !sizes || !weight_decay)) || !step_dev || !scratch_dev)
         return idm_set_error(IDM_ERR_INVALID, "adamw: null argument");
+    if ((uintptr_t)step_dev % 8 || (uintptr_t)scratch_dev % 8) return idm_set_error(IDM_ERR_INVALID, "adamw: step count and scratch must be aligned to 8 bytes");
     if (!known_dtype(cfg->param_dtype) || !known_dtype(cfg->grad_dtype)) return idm_set_error(IDM_ERR_INVALID, "adamw: unknown dtype");
     if (cfg->moment_bits != 32 && cfg->moment_bits != 8) return idm_set_error(IDM_ERR_INVALID, "adamw: moments have 32 or 8 bits");
     const bool eight = cfg->moment_bits == 8;

@@ -166,7 +166,8 @@ def test_adamw_entry_points_refuse():
                 dict(moments=0), dict(params=(1 << 20, None)), dict(params=(1 << 20, (1 << 21) + 2)), dict(grads=(1 << 22, (1 << 23) + 1)),
                 dict(params=(1 << 20, 1 << 20)), dict(params=(1 << 20, (1 << 20) + 1196)), dict(grads=(1 << 22, 1 << 20)), dict(grads=((1 << 20) + 4, 1 << 23)),
                 dict(grads=((1 << 21) - 1196, 1 << 23)), dict(grads=(1 << 20, 1 << 23), grad_dtype=1), dict(decay=(0.0, -1.0)),
-                dict(decay=(0.0, float("nan"))), dict(m=None), dict(v=8200), dict(base=(None, 32768)), dict(step=None), dict(scratch=None)):
+                dict(decay=(0.0, float("nan"))), dict(m=None), dict(v=8200), dict(base=(None, 32768)), dict(step=None), dict(scratch=None),
+                dict(step=68), dict(scratch=132)):
         assert adamw_call(**bad) == -1, bad
         assert b"adamw" in _lib.load().idm_last_error()
     lib = _lib.load()
