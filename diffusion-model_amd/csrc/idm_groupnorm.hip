@@ -1229,10 +1229,10 @@ template <typename F> int by_piece(int dtype, int pieces, F &&f)
     }
 }
 
-bool aligned16(std::initializer_list<const void *> ptrs)
+bool aligned_to(size_t n, std::initializer_list<const void *> ptrs)
 {
     for (const void *p : ptrs)
-        if ((uintptr_t)p % 16) return false;
+        if ((uintptr_t)p % n) return false;
     return true;
 }
 
@@ -1341,7 +1341,10 @@ int idm_group_norm_forward(int device, const idm_group_norm_desc *d, const void 
     const size_t need = workspace_floats(*d, false) * sizeof(float);
     if (!x_dev || !y_dev || !mean_dev || !rstd_dev || (need && !workspace_dev)) return idm_set_error(IDM_ERR_INVALID, "group norm: null argument");
     if (workspace_bytes < need) return idm_set_error(IDM_ERR_INVALID, "group norm: workspace too small");
-    const bool aligned = aligned16({x_dev, y_dev, gamma_dev, beta_dev, shift_dev});
+    if (!aligned_to(elem_bytes(d->dtype), {x_dev, y_dev}) || !aligned_to(4, {gamma_dev, beta_dev, shift_dev, mean_dev, rstd_dev}) ||
+        !aligned_to(8, {workspace_dev}))
+        return idm_set_error(IDM_ERR_INVALID, "group norm: a pointer is not aligned to its elements, or the workspace to 8 bytes");
+    const bool aligned = aligned_to(16, {x_dev, y_dev, gamma_dev, beta_dev, shift_dev});
     if (d->aligned && !aligned) return idm_set_error(IDM_ERR_INVALID, "group norm: a pointer is not aligned to 16 bytes as the descriptor says");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "group norm: no such device");
     UnitPlan u;
@@ -1372,7 +1375,10 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
         return idm_set_error(IDM_ERR_INVALID, "group norm backward: null argument");
     if (workspace_bytes < workspace_floats(*d, true) * sizeof(float))
         return idm_set_error(IDM_ERR_INVALID, "group norm backward: workspace too small");
-    const bool aligned = aligned16({dy_dev, x_dev, dx_dev, gamma_dev, beta_dev, shift_dev});
+    if (!aligned_to(elem_bytes(d->dtype), {dy_dev, x_dev, dx_dev}) || !aligned_to(8, {workspace_dev}) ||
+        !aligned_to(4, {mean_dev, rstd_dev, gamma_dev, beta_dev, shift_dev, dgamma_dev, dbeta_dev, dshift_dev}))
+        return idm_set_error(IDM_ERR_INVALID, "group norm backward: a pointer is not aligned to its elements, or the workspace to 8 bytes");
+    const bool aligned = aligned_to(16, {dy_dev, x_dev, dx_dev, gamma_dev, beta_dev, shift_dev});
     if (d->aligned && !aligned)
         return idm_set_error(IDM_ERR_INVALID, "group norm backward: a pointer is not aligned to 16 bytes as the descriptor says");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "group norm backward: no such device");

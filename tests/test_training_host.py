@@ -94,6 +94,11 @@ def test_norm_entry_points_refuse():
     assert lib.idm_group_norm_forward(0, C.byref(d), *[16] * 8, 8, None) == -1 and b"workspace" in lib.idm_last_error()
     assert lib.idm_group_norm_backward(0, C.byref(d), *[16] * 12, 8, None) == -1 and b"workspace" in lib.idm_last_error()
     assert lib.idm_group_norm_forward(0, None, *[16] * 8, 1 << 30, None) == -1
+    for n, entry in ((8, lib.idm_group_norm_forward), (12, lib.idm_group_norm_backward)):
+        for k in range(n):             # 18: no float32's address, nor the workspace's
+            args = [16] * n
+            args[k] = 18
+            assert entry(0, C.byref(d), *args, 1 << 30, None) == -1 and b"aligned" in lib.idm_last_error(), k
     d = norm_desc(aligned=1)
     assert lib.idm_group_norm_workspace(C.byref(d), 0, C.byref(size)) == 0 and size.value == 0
     for k in (0, 1, 2, 3, 4):      # x, gamma, beta, shift, y
