@@ -124,9 +124,11 @@ def test_against_the_formula(shape, groups, dtype):
 
 
 # batches that the forms for many samples take: several samples to a block, several turns of a block, a last pack that is not full,
-# groups that straddle vectors (5, 6, 12, 1 channels), one pixel, rows that are not full
+# groups that straddle vectors (5, 6, 12, 1 channels), one pixel, rows that are not full; the last two with backward blocks that
+# take more than 64 KB of a compute unit's shared memory
 MANY = [((70, 6, 6, 40), 8), ((1501, 3, 3, 16), 4), ((90, 14, 14, 192), 8), ((65, 28, 28, 96), 8), ((2051, 1, 1, 64), 8), ((777, 7, 7, 48), 8),
-        ((130, 5, 13, 64), 64), ((300, 9, 9, 128), 32), ((513, 2, 1, 8), 1), ((70, 25, 41, 32), 8)]
+        ((130, 5, 13, 64), 64), ((300, 9, 9, 128), 32), ((513, 2, 1, 8), 1), ((70, 25, 41, 32), 8),
+        ((11, 447, 912), 19), ((98, 11, 25, 160), 16)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
