@@ -569,6 +569,7 @@ struct UnitArgs {
     float inv_q, inv_qg, inv_ng, inv_seats, eps, n, inv_n;   // n: values of a group
     const float *gamma, *beta, *shift;
 };
+constexpr float kFold = 64.0f;  // |shift - mean| / deviation up to which 16-bit values are taken with their mean folded into the offset (2^-18 of gamma)
 constexpr int kTileVecs = 64;   // vectors of a tile, unless one group (or the fewest whole groups that are whole vectors) is wider
 
 // V consecutive float32 from a 16-byte aligned place
@@ -756,34 +757,50 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
             }
         });
     __syncthreads();
-    // z = (x + add) * a + sh in float32; 16-bit values, which cannot lie far from zero in units of what they resolve, take add * a
-    // into sh (its rounding is 2^-24 of |mean| / deviation, theirs 2^-9 or 2^-12 of the value)
+    // z = (x + add) * a + sh in float32.  For 16-bit values add * a goes into sh, one instruction for a value less, where |add| rstd is at most
+    // kFold: its rounding is 2^-24 of that.  In groups that are nearly constant it may be anything (a constant 60 000 with eps = 1e-3: 2e6,
+    // 0.12 of y), and add stays.
     float a[V], sh[V];
     load_chan16<V>(s.active ? g.gamma : nullptr, s.c, 1.0f, a);
     load_chan16<V>(s.active ? g.beta : nullptr, s.c, 0.0f, sh);
+    bool far = false;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const float2 t = stat[s.active ? s.sub * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0];
+        float most = 0.0f;
 #pragma unroll
         for (int j = i * PS; j < (i + 1) * PS; ++j) {
             add[j] -= t.x;
             a[j] *= t.y;
-            if constexpr (E == 2) sh[j] = __builtin_fmaf(add[j], a[j], sh[j]);
+            most = fmaxf(most, fabsf(add[j]));
+        }
+        if constexpr (E == 2) {
+            const bool fold = most * t.y <= kFold;   // (not where that is NaN)
+            far = far || (s.active && !fold);
+#pragma unroll
+            for (int j = i * PS; j < (i + 1) * PS; ++j) {
+                sh[j] = fold ? __builtin_fmaf(add[j], a[j], sh[j]) : sh[j];
+                add[j] = fold ? 0.0f : add[j];
+            }
         }
     }
     const int pitch = g.channels * E, at = (s.sub * g.pixels + s.r) * pitch + s.cq * 16;
     const auto yb = unit_buffer(y + b0 * g.pixels * g.channels + c0, kNowhere);
+    const auto finish = [&](bool add_first) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        float v[V];
-        widen<T>(raw[k], v);
+        for (int k = 0; k < NV; ++k) {
+            float v[V];
+            widen<T>(raw[k], v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(E == 2 ? v[j] : v[j] + add[j], a[j], sh[j]);
-        if (g.swish)
+            for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(add_first ? v[j] + add[j] : v[j], a[j], sh[j]);
+            if (g.swish)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] *= sigmoid(v[j]);
-        store16(yb, k < s.mine ? at + k * g.rows * pitch : kNowhere, narrow<T>(v));
-    }
+                for (int j = 0; j < V; ++j) v[j] *= sigmoid(v[j]);
+            store16(yb, k < s.mine ? at + k * g.rows * pitch : kNowhere, narrow<T>(v));
+        }
+    };
+    if (E == 4 || __any(far)) finish(true);
+    else finish(false);
 }
 
 // Backward of a unit: x and dy are read once; dz stays in the registers in float32 between the group sums and dx.  A block walks

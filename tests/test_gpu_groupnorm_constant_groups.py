@@ -1,0 +1,128 @@
+"""Group norm of groups that are constant, or constant but for one value, beside ordinary ones: there |mean| is large in units of the
+deviation sqrt(var + eps), whatever the type resolves.  Both forms (one launch; chunks, for a view that is not aligned), all types.
+
+Tolerances, per sample and group, with u = eps / 2 of the tensor's type, e = 2^-24, K = max |x + shift| or |x| of the group times its rstd:
+ * Constant groups.  The values and the values with their shift have at most 11 significant bits and a group at most 2^13 values, so every
+   sum of them is a whole multiple of their last bit below 2^24 of it: exact, and so is the mean.  u - mean is zero then and z = beta: y
+   has its rounding and the activation's 16 float32 roundings, relative to |beta|.  No K anywhere.
+ * Others: the mean is off by at most d = 16 e K in units of the deviation (sum, division, the difference), the variance by d^2 of it
+   besides its own 64 e, so xhat by d + |xhat| (64 e + d^2); z by gamma times that.
+"""
+import ctypes as C
+
+import pytest
+import torch
+
+from isingdiff import _lib, group_norm_forward
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+LARGE = {"fp32": 60000.0, "bf16": 99840.0, "fp16": 60000.0}     # 11, 8 and 11 significant bits; 1 000 has 7
+
+
+def case(shape, groups, dtype, seed, shifted, level):
+    """Groups 0, 4, ..: ordinary; 1, 5, ..: constant; 2, 6, ..: constant, another constant in every other sample; 3, 7, ..: constant but for
+    one value, one step of the type away."""
+    gen = torch.Generator().manual_seed(seed)
+    b, c = shape[0], shape[-1]
+    gc = c // groups
+    x = torch.randn(shape, generator=gen)
+    v = x.view(b, -1, groups, gc)
+    kind = torch.arange(groups) % 4
+    v[:, :, kind == 1] = level
+    v[:, :, kind == 2] = level
+    v[1::2][:, :, kind == 2] = 1000.0
+    v[:, :, kind == 3] = level
+    v[:, -1, kind == 3, 0] = level * (1 + torch.finfo(TYPES[dtype]).eps)
+    shift = None
+    if shifted:     # constant groups stay constant
+        shift = 0.5 * torch.randn(b, groups, gc, generator=gen)
+        shift[:, kind > 0] = 512.0
+        shift = shift.view(b, c).cuda()
+    gamma, beta = 1 + 0.2 * torch.randn(c, generator=gen), 0.2 * torch.randn(c, generator=gen)
+    return x.to(TYPES[dtype]).cuda(), gamma.cuda(), beta.cuda(), shift, torch.randn(shape, generator=gen).to(TYPES[dtype]).cuda()
+
+
+def unaligned(t):
+    """The same values with a pitch and an offset that allow no vectors."""
+    wide = torch.zeros(t.shape[:-1] + (t.shape[-1] + 3,), dtype=t.dtype, device=t.device)
+    wide[..., 1:1 + t.shape[-1]] = t
+    return wide[..., 1:1 + t.shape[-1]]
+
+
+def in_one_launch(x, groups):
+    """Whether the aligned forward call takes the one-launch form: it then needs no workspace."""
+    b, c = x.shape[0], x.shape[-1]
+    n = x.numel() // (b * c)
+    d = _lib.GroupNormDesc(dtype={torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[x.dtype], activation=1, batch=b, pixels=n, channels=c,
+                           groups=groups, x_sample=n * c, x_pixel=c, shift_sample=c, eps=1e-3, aligned=1)
+    size = C.c_size_t()
+    assert _lib.load().idm_group_norm_workspace(C.byref(d), 0, C.byref(size)) == 0
+    return size.value == 0
+
+
+def over(name, got, want, tol):
+    off = (got.detach().cpu().double() - want).abs() - tol
+    bad = ~(off <= 0)
+    assert not bool(bad.any()), f"{name}: {int(bad.sum())} of {bad.numel()} over their tolerance, the worst by {float(off.max()):.3g}"
+
+
+class Truth:
+    """The formulas in 64 bits, grouped (sample, pixel, group, channel of the group), and how far xhat may be off."""
+
+    def __init__(self, x, gamma, beta, shift, groups, act, eps):
+        b, c = x.shape[0], x.shape[-1]
+        self.groups, self.gc, self.u = groups, c // groups, torch.finfo(x.dtype).eps / 2
+        self.tiny = 6e-8 if x.dtype == torch.float16 else 0.0        # half the spacing of fp16 below its normal numbers
+        xs, self.g, self.bt = self.grouped(x), self.row(gamma), self.row(beta)
+        us = xs if shift is None else xs + shift.cpu().double().view(b, 1, groups, self.gc)
+        self.constant = (us == us[:, :1, :, :1]).all(3, keepdim=True).all(1, keepdim=True)
+        assert bool(self.constant[:, :, torch.arange(groups) % 4 == 1].all())
+        self.mean = torch.where(self.constant, us[:, :1, :, :1], us.mean((1, 3), keepdim=True))
+        self.rstd = 1 / torch.sqrt((us - self.mean).square().mean((1, 3), keepdim=True) + eps)
+        self.xhat = (us - self.mean) * self.rstd
+        self.z = self.xhat * self.g + self.bt
+        self.s = torch.sigmoid(self.z) if act == "swish" else torch.ones_like(self.z)
+        self.top = us.abs().amax((1, 3), keepdim=True)
+        k = torch.maximum(us.abs(), xs.abs()).amax((1, 3), keepdim=True) * self.rstd
+        self.d = torch.where(self.constant, 0.0, 16 * E * k)
+        self.off = self.d + self.xhat.abs() * (64 * E + self.d * self.d)
+
+    def grouped(self, t):
+        return t.detach().cpu().double().reshape(t.shape[0], -1, self.groups, self.gc)
+
+    def row(self, t):
+        return t.detach().cpu().double().view(self.groups, self.gc)
+
+    def forward(self, y, m, r):
+        y, m, r = self.grouped(y), m.cpu().double().view(self.mean.shape), r.cpu().double().view(self.mean.shape)
+        over("mean", m, self.mean, torch.where(self.constant, 0.0, 16 * E * self.top))
+        over("rstd", r, self.rstd, (64 * E + self.d * self.d) * self.rstd)
+        want = self.z * self.s
+        over("y", y, want, self.u * want.abs() + 1.1 * (self.off * self.g.abs() + 16 * E * (self.z.abs() + self.bt.abs())) + self.tiny)
+
+
+# groups of whole vectors, of half vectors, of single values (5, 1 channels); few and many samples, several to a block; groups have at most 2^13
+# values
+SHAPES = [((3, 20, 20, 64), 4), ((2, 12, 11, 48), 4), ((5, 9, 7, 40), 8), ((3, 14, 13, 32), 32), ((70, 6, 6, 96), 8), ((1030, 3, 3, 64), 8), ((6, 28, 28, 32), 4)]
+
+
+def cases(shape, groups, dtype, form):
+    for i, (level, eps) in enumerate(((1000.0, 1e-3), (LARGE[dtype], 1e-3), (1000.0, 1e-5), (LARGE[dtype], 1e-5))):
+        x, gamma, beta, shift, dy = case(shape, groups, dtype, 7 + i, i % 2 == 1, level)
+        if form == "chunks":
+            x, dy = unaligned(x), unaligned(dy)
+        else:
+            assert in_one_launch(x, groups)
+        yield x, gamma, beta, shift, dy, ["swish", "none"][(i + sum(shape)) % 2], eps
+
+
+@pytest.mark.parametrize("form", ["one launch", "chunks"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,groups", SHAPES)
+def test_constant_groups_beside_others(shape, groups, dtype, form):
+    for x, gamma, beta, shift, _, act, eps in cases(shape, groups, dtype, form):
+        got = group_norm_forward(x, gamma, beta, groups, shift=shift, eps=eps, activation=act)
+        Truth(x, gamma, beta, shift, groups, act, eps).forward(*got)
