@@ -4,16 +4,17 @@ deviation sqrt(var + eps), whatever the type resolves.  Both forms (one launch; 
 Tolerances, per sample and group, with u = eps / 2 of the tensor's type, e = 2^-24, K = max |x + shift| or |x| of the group times its rstd:
  * Constant groups.  The values and the values with their shift have at most 11 significant bits and a group at most 2^13 values, so every
    sum of them is a whole multiple of their last bit below 2^24 of it: exact, and so is the mean.  u - mean is zero then and z = beta: y
-   has its rounding and the activation's 16 float32 roundings, relative to |beta|.  No K anywhere.
+   has its rounding and the activation's 16 float32 roundings, relative to |beta|; dgamma is a sum of zeros; dx = rstd (dz gamma - A) has
+   its rounding and a sum of at most 64 roundings in line.  No K anywhere.
  * Others: the mean is off by at most d = 16 e K in units of the deviation (sum, division, the difference), the variance by d^2 of it
-   besides its own 64 e, so xhat by d + |xhat| (64 e + d^2); z by gamma times that.
+   besides its own 64 e, so xhat by d + |xhat| (64 e + d^2); z by gamma times that and dz by at most |dy| gamma / 2 times that.
 """
 import ctypes as C
 
 import pytest
 import torch
 
-from isingdiff import _lib, group_norm_forward
+from isingdiff import _lib, group_norm_backward, group_norm_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -85,6 +86,7 @@ class Truth:
         self.xhat = (us - self.mean) * self.rstd
         self.z = self.xhat * self.g + self.bt
         self.s = torch.sigmoid(self.z) if act == "swish" else torch.ones_like(self.z)
+        self.slope = self.s * (1 + self.z * (1 - self.s)) if act == "swish" else self.s
         self.top = us.abs().amax((1, 3), keepdim=True)
         k = torch.maximum(us.abs(), xs.abs()).amax((1, 3), keepdim=True) * self.rstd
         self.d = torch.where(self.constant, 0.0, 16 * E * k)
@@ -102,6 +104,28 @@ class Truth:
         over("rstd", r, self.rstd, (64 * E + self.d * self.d) * self.rstd)
         want = self.z * self.s
         over("y", y, want, self.u * want.abs() + 1.1 * (self.off * self.g.abs() + 16 * E * (self.z.abs() + self.bt.abs())) + self.tiny)
+
+    def backward(self, dy, gx, gg, gb, gs):
+        each, off, xhat, rstd = (1, 3), self.off, self.xhat, self.rstd
+        dy = self.grouped(dy)
+        dz = dy * self.slope
+        dg = dz * self.g
+        first, second = dg.mean(each, keepdim=True), (dg * xhat).mean(each, keepdim=True)
+        dx = rstd * (dg - first - second * xhat)
+        off_dz = dy.abs() * (16 * E + 0.5 * self.g.abs() * off)
+        off_dg = off_dz * self.g.abs()
+        off_second = dg.abs().mean(each, keepdim=True) * off.amax(each, keepdim=True) + off_dg.mean(each, keepdim=True) * xhat.abs().amax(each, keepdim=True)
+        off_second = torch.where(self.constant, 0.0, off_second)
+        off_dx = rstd * (64 * E * (1 + xhat.abs()) * dg.abs().amax(each, keepdim=True) + off_dg + off_dg.mean(each, keepdim=True) + off_second * xhat.abs() +
+                         second.abs() * off) + self.d * self.d * dx.abs()
+        over("dx", self.grouped(gx), dx, self.u * dx.abs() + off_dx + self.tiny)
+        assert not bool(self.row(gg)[torch.arange(self.groups) % 4 == 1].any()), "dgamma of constant groups"
+        many = 512 * E
+        over("dgamma", self.row(gg), (dz * xhat).sum((0, 1)), (many * (dz * xhat).abs() + dz.abs() * off + off_dz * xhat.abs()).sum((0, 1)))
+        over("dbeta", self.row(gb), dz.sum((0, 1)), (many * dz.abs() + off_dz).sum((0, 1)))
+        if gs is not None:
+            terms = rstd * (dg.abs() + first.abs() + second.abs() * xhat.abs())
+            over("dshift", gs.cpu().double().view(-1, self.groups, self.gc), dx.sum(1), (many * terms + off_dx).sum(1))
 
 
 # groups of whole vectors, of half vectors, of single values (5, 1 channels); few and many samples, several to a block; groups have at most 2^13
@@ -126,3 +150,13 @@ def test_constant_groups_beside_others(shape, groups, dtype, form):
     for x, gamma, beta, shift, _, act, eps in cases(shape, groups, dtype, form):
         got = group_norm_forward(x, gamma, beta, groups, shift=shift, eps=eps, activation=act)
         Truth(x, gamma, beta, shift, groups, act, eps).forward(*got)
+
+
+@pytest.mark.parametrize("form", ["one launch", "chunks"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,groups", SHAPES)
+def test_gradients_of_constant_groups_beside_others(shape, groups, dtype, form):
+    for x, gamma, beta, shift, dy, act, eps in cases(shape, groups, dtype, form):
+        _, m, r = group_norm_forward(x, gamma, beta, groups, shift=shift, eps=eps, activation=act)
+        got = group_norm_backward(dy, x, m, r, gamma, beta, groups, shift=shift, activation=act)
+        Truth(x, gamma, beta, shift, groups, act, eps).backward(dy, *got)
