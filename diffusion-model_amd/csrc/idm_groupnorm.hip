@@ -569,7 +569,6 @@ struct UnitArgs {
     float inv_q, inv_qg, inv_ng, inv_seats, eps, n, inv_n;   // n: values of a group
     const float *gamma, *beta, *shift;
 };
-constexpr float kFold = 64.0f;  // |shift - mean| / deviation up to which 16-bit values are taken with their mean folded into the offset (2^-18 of gamma)
 constexpr int kTileVecs = 64;   // vectors of a tile, unless one group (or the fewest whole groups that are whole vectors) is wider
 
 // V consecutive float32 from a 16-byte aligned place
@@ -757,50 +756,33 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
             }
         });
     __syncthreads();
-    // z = (x + add) * a + sh in float32.  For 16-bit values add * a goes into sh, one instruction for a value less, where |add| rstd is at most
-    // kFold: its rounding is 2^-24 of that.  In groups that are nearly constant it may be anything (a constant 60 000 with eps = 1e-3: 2e6,
-    // 0.12 of y), and add stays.
+    // z = (x + add) * a + sh in float32.  (Never add * a folded into sh, one instruction for a value less: its rounding is 2^-24 of |mean| rstd,
+    // which has no bound where a group is nearly constant, 0.12 of y for 60 000 and eps = 1e-3.  1 024 x 784 x 96 bf16 89 us, folded 88.)
     float a[V], sh[V];
     load_chan16<V>(s.active ? g.gamma : nullptr, s.c, 1.0f, a);
     load_chan16<V>(s.active ? g.beta : nullptr, s.c, 0.0f, sh);
-    bool far = false;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const float2 t = stat[s.active ? s.sub * g.ng + quotient(s.cq * P + i, g.inv_qg) : 0];
-        float most = 0.0f;
 #pragma unroll
         for (int j = i * PS; j < (i + 1) * PS; ++j) {
             add[j] -= t.x;
             a[j] *= t.y;
-            most = fmaxf(most, fabsf(add[j]));
-        }
-        if constexpr (E == 2) {
-            const bool fold = most * t.y <= kFold;   // (not where that is NaN)
-            far = far || (s.active && !fold);
-#pragma unroll
-            for (int j = i * PS; j < (i + 1) * PS; ++j) {
-                sh[j] = fold ? __builtin_fmaf(add[j], a[j], sh[j]) : sh[j];
-                add[j] = fold ? 0.0f : add[j];
-            }
         }
     }
     const int pitch = g.channels * E, at = (s.sub * g.pixels + s.r) * pitch + s.cq * 16;
     const auto yb = unit_buffer(y + b0 * g.pixels * g.channels + c0, kNowhere);
-    const auto finish = [&](bool add_first) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            float v[V];
-            widen<T>(raw[k], v);
+    for (int k = 0; k < NV; ++k) {
+        float v[V];
+        widen<T>(raw[k], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(add_first ? v[j] + add[j] : v[j], a[j], sh[j]);
-            if (g.swish)
+        for (int j = 0; j < V; ++j) v[j] = __builtin_fmaf(v[j] + add[j], a[j], sh[j]);
+        if (g.swish)
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] *= sigmoid(v[j]);
-            store16(yb, k < s.mine ? at + k * g.rows * pitch : kNowhere, narrow<T>(v));
-        }
-    };
-    if (E == 4 || __any(far)) finish(true);
-    else finish(false);
+            for (int j = 0; j < V; ++j) v[j] *= sigmoid(v[j]);
+        store16(yb, k < s.mine ? at + k * g.rows * pitch : kNowhere, narrow<T>(v));
+    }
 }
 
 // Backward of a unit: x and dy are read once; dz stays in the registers in float32 between the group sums and dx.  A block walks
