@@ -679,14 +679,15 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
 #pragma unroll
         for (int k = 0; k < NV; ++k) raw[k] = load16(xb, k < s.mine ? at + k * g.rows * pitch : kNowhere);
     }
-    float add[V], mean[P], m2[P];
+    float add[V], mean[P] = {}, m2[P] = {};
     load_chan16<V>(g.shift && s.active ? g.shift + s.b * g.shift_sample : nullptr, s.c, 0.0f, add);
     // The thread's own mean and squared distances from it, then the group's from all of its threads'.  A sum of squares around zero
     // would lose the variance of values far from it, so the distances are summed; only where 16-bit values come without a shift,
     // and the thread's mean turns out to be within four of its deviations, do sum and sum of squares (two instructions for two
-    // values instead of eight) stand: that loses less than five bits.
+    // values instead of eight) stand: that loses less than five bits.  Each piece decides for itself: what one group holds does not change
+    // another's bits.
     const float own = (float)(s.mine ? s.mine * PS : 1), share = __builtin_amdgcn_rcpf(own);
-    bool sure = false;
+    bool sure[P] = {}, all = false;
     if constexpr (E == 2 && P <= 2) {
         if (!g.shift) {
             float sum[P], squares[P];
@@ -694,32 +695,34 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
             for (int i = 0; i < P; ++i) sum[i] = squares[i] = 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) add_pairs<P>(raw[k], T{}, sum, squares);
-            sure = true;
+            all = true;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 mean[i] = over(sum[i], own, share);
                 m2[i] = squares[i] - sum[i] * mean[i];
-                sure = sure && squares[i] < 0x1p126f && !(m2[i] * 16.0f < sum[i] * mean[i]);   // (squares that overflow, too)
+                sure[i] = squares[i] < 0x1p126f && !(m2[i] * 16.0f < sum[i] * mean[i]);   // (not where squares overflow)
+                all = all && sure[i];
             }
         }
     }
-    if (!sure) {
+    if (!all) {
+        float mean_[P], m2_[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            mean[i] = m2[i] = 0.0f;
+            mean_[i] = m2_[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < PS; ++j) mean[i] += add[i * PS + j];
-            mean[i] *= (float)s.mine;
+            for (int j = 0; j < PS; ++j) mean_[i] += add[i * PS + j];
+            mean_[i] *= (float)s.mine;
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             float v[V];
             widen<T>(raw[k], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) mean[j / PS] += v[j];
+            for (int j = 0; j < V; ++j) mean_[j / PS] += v[j];
         }
 #pragma unroll
-        for (int i = 0; i < P; ++i) mean[i] = over(mean[i], own, share);
+        for (int i = 0; i < P; ++i) mean_[i] = over(mean_[i], own, share);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (k >= s.mine) continue;
@@ -727,9 +730,14 @@ __global__ __launch_bounds__(TH) void gn_unit_forward_kernel(UnitArgs g, const T
             widen<T>(raw[k], v);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = v[j] + (add[j] - mean[j / PS]);
-                m2[j / PS] = __builtin_fmaf(d, d, m2[j / PS]);
+                const float d = v[j] + (add[j] - mean_[j / PS]);
+                m2_[j / PS] = __builtin_fmaf(d, d, m2_[j / PS]);
             }
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            mean[i] = sure[i] ? mean[i] : mean_[i];
+            m2[i] = sure[i] ? m2[i] : m2_[i];
         }
     }
 #pragma unroll

@@ -160,3 +160,34 @@ def test_gradients_of_constant_groups_beside_others(shape, groups, dtype, form):
         _, m, r = group_norm_forward(x, gamma, beta, groups, shift=shift, eps=eps, activation=act)
         got = group_norm_backward(dy, x, m, r, gamma, beta, groups, shift=shift, activation=act)
         Truth(x, gamma, beta, shift, groups, act, eps).backward(dy, *got)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_constant_group_leaves_the_others_bits(dtype):
+    """What a group's neighbours (in the vector, in the wavefront, in the pack) hold does not change its result."""
+    for shape, groups in SHAPES:
+        x, gamma, beta, _, dy = case(shape, groups, dtype, 3, False, 1000.0)
+        plain = torch.randn(shape, generator=torch.Generator().manual_seed(5)).to(TYPES[dtype]).cuda()
+        keep = torch.zeros(groups, dtype=torch.bool, device="cuda")
+        keep[::4] = True
+        keep = keep.repeat_interleave(shape[-1] // groups)
+        a, b = torch.where(keep, plain, x), plain
+        ya, ma, ra = group_norm_forward(a, gamma, beta, groups)
+        yb, mb, rb = group_norm_forward(b, gamma, beta, groups)
+        assert torch.equal(ya[..., keep], yb[..., keep])
+        da, db = group_norm_backward(dy, a, ma, ra, gamma, beta, groups), group_norm_backward(dy, b, mb, rb, gamma, beta, groups)
+        assert torch.equal(da[0][..., keep], db[0][..., keep])
+        assert torch.equal(da[1][keep], db[1][keep]) and torch.equal(da[2][keep], db[2][keep])
+
+
+@pytest.mark.parametrize("power", [-60, -66])
+def test_bfloat16_values_whose_squares_are_subnormal(power):
+    """eps = 0 and deviations of 2^power: squares of 2^-120 and 2^-132, the latter below the normal float32 numbers, where they keep 17 bits:
+    a relative 2^-18 of the variance, half of it in rstd."""
+    gen = torch.Generator().manual_seed(9)
+    x = (torch.randn(4, 12, 12, 32, generator=gen).sign() * 2.0 ** power).to(torch.bfloat16).cuda()
+    _, mean, rstd = group_norm_forward(x, None, None, 4, eps=0.0, activation="none")
+    g = x.cpu().double().reshape(4, 144, 4, 8)
+    m, v = g.mean((1, 3)), g.var((1, 3), correction=0)
+    over("mean", mean, m, 64 * E * 2.0 ** power)
+    over("rstd", rstd, v.rsqrt(), (64 * E + 2.0 ** -18) * v.rsqrt())
