@@ -301,8 +301,11 @@ try {
     if (!(cfg->lr >= 0) || std::isinf(cfg->lr) || !(cfg->beta1 >= 0 && cfg->beta1 < 1) || !(cfg->beta2 >= 0 && cfg->beta2 < 1) ||
         !(cfg->eps >= 0) || std::isinf(cfg->eps))
         return idm_set_error(IDM_ERR_INVALID, "adamw: lr and eps must be finite and not negative, the betas in [0, 1)");
-    int64_t total = 0, work = 0;                // entries of the moments, workgroups
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    int64_t total = 0, work = 0, tensors = 0;   // entries of the moments, workgroups, tensors with gradients
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;   // what the step writes
+    const auto writes = [&](const void *p, size_t bytes) {
+        if (bytes) spans.push_back({(uintptr_t)p, (uintptr_t)p + bytes});
+    };
     const size_t pb = cfg->param_dtype == IDM_DT_F32 ? 4 : 2, gb = cfg->grad_dtype == IDM_DT_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {
         if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 40)) return idm_set_error(IDM_ERR_INVALID, "adamw: tensor size out of range");
@@ -313,27 +316,34 @@ try {
         if (!params_dev[i]) return idm_set_error(IDM_ERR_INVALID, "adamw: null parameter");
         if ((uintptr_t)params_dev[i] % pb || (uintptr_t)grads_dev[i] % gb) return idm_set_error(IDM_ERR_INVALID, "adamw: misaligned tensor");
         work += (sizes[i] + CHUNK - 1) / CHUNK;
-        spans.push_back({(uintptr_t)params_dev[i], (uintptr_t)params_dev[i] + (size_t)sizes[i] * pb});
+        writes(params_dev[i], (size_t)sizes[i] * pb);
+        ++tensors;
     }
     if (total / BLOCK > 0xffffffff) return idm_set_error(IDM_ERR_INVALID, "adamw: more than 2^40 entries");
     if (total != moments) return idm_set_error(IDM_ERR_INVALID, "adamw: the moments were made for other tensors (each takes its size rounded up to 256 entries)");
+    if (total && (!m_dev || !v_dev || (eight && (!m_base_dev || !v_base_dev)))) return idm_set_error(IDM_ERR_INVALID, "adamw: null moments");
+    if ((uintptr_t)m_dev % 16 || (uintptr_t)v_dev % 16 || (eight && ((uintptr_t)m_base_dev % 2 || (uintptr_t)v_base_dev % 2)))
+        return idm_set_error(IDM_ERR_INVALID, "adamw: moments must be aligned to 16 bytes, their bases to 2");
+    for (const void *p : {(const void *)m_dev, (const void *)v_dev}) writes(p, (size_t)total * (eight ? 1 : 4));
+    for (const void *p : {(const void *)m_base_dev, (const void *)v_base_dev}) writes(p, eight ? (size_t)(total / BLOCK) * 2 : 0);
+    writes(step_dev, 8);
+    writes(scratch_dev, 16);
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
-        if (spans[i].first < spans[i - 1].second) return idm_set_error(IDM_ERR_INVALID, "adamw: two parameters share memory");
-    for (int64_t i = 0; i < n_tensors; ++i) {   // workgroups read gradients while others write parameters
+        if (spans[i].first < spans[i - 1].second)
+            return idm_set_error(IDM_ERR_INVALID, "adamw: two of parameters, moments, bases, step count and scratch share memory");
+    for (int64_t i = 0; i < n_tensors; ++i) {   // workgroups read gradients while others write parameters and state
         if (!sizes[i] || !grads_dev[i]) continue;
         const uintptr_t lo = (uintptr_t)grads_dev[i], hi = lo + (size_t)sizes[i] * gb;
         auto after = std::lower_bound(spans.begin(), spans.end(), std::make_pair(hi, (uintptr_t)0));   // the first one from hi on
         for (; after != spans.begin() && (after - 1)->second > lo; --after)
             if ((after - 1)->first != lo || params_dev[i] != grads_dev[i] || pb != gb)
-                return idm_set_error(IDM_ERR_INVALID, "adamw: a gradient shares memory with a parameter");
+                return idm_set_error(IDM_ERR_INVALID, "adamw: a gradient shares memory with a parameter or the state");
     }
-    if (total && (!m_dev || !v_dev || (eight && (!m_base_dev || !v_base_dev)))) return idm_set_error(IDM_ERR_INVALID, "adamw: null moments");
-    if ((uintptr_t)m_dev % 16 || (uintptr_t)v_dev % 16) return idm_set_error(IDM_ERR_INVALID, "adamw: moments must be aligned to 16 bytes");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "adamw: no such device");
     hipStream_t s = (hipStream_t)stream;
     const Clock clock = {step_dev, cfg->lr, std::log2(cfg->beta1), std::log2(cfg->beta2)};
-    Coef *coef = work && spans.size() <= (size_t)TENSORS && work <= kOnce ? nullptr : (Coef *)scratch_dev;
+    Coef *coef = work && tensors <= TENSORS && work <= kOnce ? nullptr : (Coef *)scratch_dev;
     if (coef) hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, s, clock, coef);
     const float b1 = (float)cfg->beta1, c1 = (float)(1 - cfg->beta1), b2 = (float)cfg->beta2, c2 = (float)(1 - cfg->beta2);
     // (50 M float32: 267 us, 278 through the cache; 33 M: 140 and 190; below the limit it costs up to a twentieth, and codes gain nothing)
@@ -392,6 +402,12 @@ int idm_adamw_moments(int device, const uint8_t *m_dev, const uint8_t *v_dev, co
     if (!m_dev || !v_dev || !m_base_dev || !v_base_dev || !m_out_dev || !v_out_dev) return idm_set_error(IDM_ERR_INVALID, "adamw: null argument");
     if ((uintptr_t)m_dev % 16 || (uintptr_t)v_dev % 16 || (uintptr_t)m_out_dev % 16 || (uintptr_t)v_out_dev % 16)
         return idm_set_error(IDM_ERR_INVALID, "adamw: moments must be aligned to 16 bytes");
+    const size_t n = (size_t)moments, bytes[6] = {n, n, n / BLOCK * 2, n / BLOCK * 2, 4 * n, 4 * n};
+    const void *const at[6] = {m_dev, v_dev, m_base_dev, v_base_dev, m_out_dev, v_out_dev};
+    for (int i = 4; i < 6; ++i)
+        for (int k = 0; k < i; ++k)
+            if ((uintptr_t)at[i] < (uintptr_t)at[k] + bytes[k] && (uintptr_t)at[k] < (uintptr_t)at[i] + bytes[i])
+                return idm_set_error(IDM_ERR_INVALID, "adamw: the moments' values share memory with their codes or each other");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "adamw: no such device");
     hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)((moments / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, m_dev, v_dev,
                        m_base_dev, v_base_dev, m_out_dev, v_out_dev, moments);

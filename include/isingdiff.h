@@ -387,8 +387,9 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
 /* One AdamW step over n_tensors tensors: t = *step_dev + 1 (written back), and per entry
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * params / grads / sizes / weight_decay: host arrays of n_tensors device pointers, entry counts and decays; a NULL gradient leaves
- * its tensor and moments as they are.  Gradients and parameters are dense; parameters must not share memory,
- * nor a gradient with a parameter (but for its own, entry by entry).
+ * its tensor and moments as they are.  Gradients and parameters are dense.  What a step writes
+ * (parameters, moments, bases, step count, scratch) must not share memory, nor a gradient with any of it (but for its own parameter, entry
+ * by entry): such calls are refused.
  * Moments: tensor i's begin at the sum of the sizes before it, each rounded up to IDM_ADAMW_BLOCK entries; `moments` is that sum
  * over all tensors.  moment_bits 32: m_dev, v_dev float32, bases unused.  8: bytes, with one int16 base per block of
  * IDM_ADAMW_BLOCK entries; code c > 0 stands for the float32 with bits (c + base) << 20 (m: bit 7 is the sign), rounded with a
@@ -407,7 +408,7 @@ int idm_adamw_step(int device, const idm_adamw_cfg *cfg, int64_t n_tensors, void
                    const void *const *grads_dev, const int64_t *sizes, const float *weight_decay, void *m_dev, void *v_dev,
                    int16_t *m_base_dev, int16_t *v_base_dev, int64_t moments, int64_t *step_dev, void *scratch_dev, void *stream);
 
-/* The float32 values that 8-bit moments stand for: `moments` entries each. */
+/* The float32 values that 8-bit moments stand for: `moments` entries each, in memory of their own. */
 int idm_adamw_moments(int device, const uint8_t *m_dev, const uint8_t *v_dev, const int16_t *m_base_dev,
                       const int16_t *v_base_dev, float *m_out_dev, float *v_out_dev, int64_t moments, void *stream);
 
