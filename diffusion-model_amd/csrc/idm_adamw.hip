@@ -49,7 +49,7 @@ struct Table {
 };
 
 struct Coef {
-    float size, root;                       // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    float size, root;                       // lr / (1 - b1^t), -1 where the count is none; 1 / sqrt(1 - b2^t)
     uint32_t t, unused;
 };
 
@@ -61,18 +61,20 @@ struct Clock {
 
 DEVI Coef coef_of(int64_t t, const Clock &c)
 {
+    if (t <= 0) return {-1.0f, 0.0f, 0, 0};   // the count before it was negative
     return {(float)(c.lr / (1.0 - exp2((double)t * c.log1))), (float)(1.0 / sqrt(1.0 - exp2((double)t * c.log2))), (uint32_t)t, 0};
 }
 
 // A step of one launch of at most kOnce workgroups counts itself: they all read the count, and each adds one to the bits above it when
-// // it has done so; the last of them moves the count on and clears those bits.  Larger steps begin with a kernel of one thread: the
-// additions go one after the other (one workgroup 3.8 us instead of 4.8 and 3 us less of host, 198 of them 8.2 and 8.5, 960 27 and 21).
+// it has done so; the last of them moves the count on and clears those bits.  (A negative count stays one until somebody adds, and nobody
+// who sees one adds.)  Larger steps begin with a kernel of one thread: the additions go one after the other (one workgroup 3.8 us instead
+// of 4.8 and 3 us less of host, 198 of them 8.2 and 8.5, 960 27 and 21).
 constexpr int kOnce = 256, kCountBits = 53;
 
 __global__ void adamw_begin_kernel(Clock clock, Coef *c)
 {
-    const int64_t t = *clock.step + 1;
-    *clock.step = t;
+    const int64_t t = *clock.step < 0 ? 0 : *clock.step + 1;
+    if (t) *clock.step = t;
     *c = coef_of(t, clock);
 }
 
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, Clock clock, cons
     const GT *g = (const GT *)tab.g[k];
     const int64_t n = tab.n[k], at = (int64_t)tab.at[k] * BLOCK, i0 = (int64_t)(chunk - tab.first[k]) * CHUNK;
     const bool aligned = ((uintptr_t)p % (N * sizeof(PT)) | (uintptr_t)g % (N * sizeof(GT))) == 0;
-    const int64_t steps = coef ? 0 : (*clock.step & (((int64_t)1 << kCountBits) - 1)) + 1;
+    const int64_t count = coef ? 0 : *clock.step, steps = count < 0 ? 0 : (count & (((int64_t)1 << kCountBits) - 1)) + 1;
     const Coef now = coef ? *coef : coef_of(steps, clock);
     const float keep = tab.keep[k], size = now.size, root = now.root;
     const uint32_t t = now.t;
@@ -171,6 +173,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, Clock clock, cons
         load_entries<PT, N>(p, i, n, full, pv);
         load_entries<GT, N>(g, i, n, full, gv);
         const int64_t w = (at + i) / BLOCK;    // the block among the moments
+        if (size < 0.0f) break;                // (all threads or none; here, where the loads are on their way)
         if constexpr (EIGHT) {
             const u32x2 cm = take<FAR>((const u32x2 *)((const uint8_t *)m_all + at + i)), cv = take<FAR>((const u32x2 *)((const uint8_t *)v_all + at + i));
             const int bm = m_base[w], bv = v_base[w];
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table tab, Clock clock, cons
             put<FAR>((f32x4 *)((float *)v_all + at + i), f32x4{v[0], v[1], v[2], v[3]});
         }
     }
-    if (!coef) {
+    if (!coef && size >= 0.0f) {
         __syncthreads();   // all wavefronts have read the count
         if (threadIdx.x == 0) {
             typedef unsigned long long word;

@@ -81,5 +81,7 @@ class AdamW:
         for k, t in self.state.items():
             if state[k].shape != t.shape or state[k].dtype != t.dtype:
                 raise ValueError(f"state[{k!r}] does not fit these parameters")
+        if not 0 <= int(state["step"]) < 2 ** 53 - 1:
+            raise ValueError("state['step'] must be a count of steps")
         for k, t in self.state.items():
             t.copy_(state[k])

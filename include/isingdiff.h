@@ -394,8 +394,9 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
  * over all tensors.  moment_bits 32: m_dev, v_dev float32, bases unused.  8: bytes, with one int16 base per block of
  * IDM_ADAMW_BLOCK entries; code c > 0 stands for the float32 with bits (c + base) << 20 (m: bit 7 is the sign), rounded with a
  * dither that is equidistributed over entries and steps.  All zero is the state of step 0 in both forms.
- * step_dev: one int64, below 2^53 (a running step uses the bits above as a counter).  scratch_dev: 16 bytes.  The tables are copied at the call: the host arrays may be reused at once, and a captured call replays
- * with the pointers, lr and decays that it was captured with while the step count goes on. */
+ * step_dev: one int64 from 0 on, below 2^53 - 1 (a running step uses the bits above as a counter); with a negative one a step
+ * writes nothing.  scratch_dev: 16 bytes.  The tables are copied at the call: the host arrays may be reused at once, and a captured
+ * call replays with the pointers, lr and decays that it was captured with while the step count goes on. */
 #define IDM_ADAMW_BLOCK 256
 
 typedef struct {
