@@ -349,6 +349,8 @@ try {
     Coef *coef = work && tensors <= TENSORS && work <= kOnce ? nullptr : (Coef *)scratch_dev;
     if (coef) hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, s, clock, coef);
     const float b1 = (float)cfg->beta1, c1 = (float)(1 - cfg->beta1), b2 = (float)cfg->beta2, c2 = (float)(1 - cfg->beta2);
+    // 1 / x of a subnormal x is infinite, and 0 times that no number.  Above zero a root is at least 2^-75, so eps does not count down there
+    const float eps = cfg->eps > 0 ? std::max((float)cfg->eps, 0x1p-126f) : 0.0f;
     // (50 M float32: 267 us, 278 through the cache; 33 M: 140 and 190; below the limit it costs up to a twentieth, and codes gain nothing)
     const bool far = !eight && total * (int64_t)(pb + gb + 8) > (int64_t)1 << 28;
     int64_t at = 0;
@@ -362,7 +364,7 @@ try {
             using PT = decltype(p);
             using GT = decltype(g);
             auto kernel = eight ? &adamw_kernel<PT, GT, true, false> : far ? &adamw_kernel<PT, GT, false, true> : &adamw_kernel<PT, GT, false, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(256), 0, s, tab, clock, (const Coef *)coef, b1, c1, b2, c2, (float)cfg->eps, m_dev,
+            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(256), 0, s, tab, clock, (const Coef *)coef, b1, c1, b2, c2, eps, m_dev,
                                v_dev, m_base_dev, v_base_dev);
             return IDM_OK;
         };

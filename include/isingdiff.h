@@ -386,6 +386,7 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
 
 /* One AdamW step over n_tensors tensors: t = *step_dev + 1 (written back), and per entry
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * where an eps between 0 and 2^-126 counts as 2^-126.
  * params / grads / sizes / weight_decay: host arrays of n_tensors device pointers, entry counts and decays; a NULL gradient leaves
  * its tensor and moments as they are.  Gradients and parameters are dense.  What a step writes
  * (parameters, moments, bases, step count, scratch) must not share memory, nor a gradient with any of it (but for its own parameter, entry

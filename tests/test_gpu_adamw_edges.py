@@ -40,3 +40,20 @@ def test_counts_that_are_none_are_not_loaded():
     opt.params[0].grad = torch.ones(5, device="cuda")
     opt.step()
     assert int(opt.state["step"]) == 2 ** 53 - 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-38, 1e-42, 1e-50, 1e-300])
+def test_an_eps_below_the_normal_float32_numbers(eps, bits):
+    """0 / (0 + eps) is 0 for every eps above zero.  Elsewhere the root of a moment is at least 2^-75 (codes: 2^-64), where no such eps counts."""
+    p = torch.linspace(-1, 1, 512, device="cuda")
+    q, g = p.clone(), torch.zeros(512, device="cuda")
+    g[::2] = torch.linspace(-1e-3, 1e-3, 256, device="cuda")
+    g[2] = 1e-20
+    s, r = adamw_state([p], bits), adamw_state([q], bits)
+    for _ in range(3):
+        before = p.clone()
+        adamw_step([p], [g], s, eps=eps, weight_decay=0.0)
+        adamw_step([q], [g], r, eps=2.0 ** -100, weight_decay=0.0)
+        assert torch.equal(p[1::2], before[1::2])
+    assert torch.equal(p, q) and all(torch.equal(s[k], r[k]) for k in s)
