@@ -211,9 +211,10 @@ PyObject *group_norm_forward(PyObject *, PyObject *const *arg, Py_ssize_t)
 {
     return guarded([&]() -> PyObject * {
         const double eps = number(arg[5]);
+        if (!(eps >= 0) || !std::isfinite((float)eps) || (eps > 0 && (float)eps == 0))
+            refuse("eps must be finite, not negative, and above zero in float32 if it is above zero");
         Norm a = norm_args(arg[0], arg[1], arg[2], arg[3], arg[4], arg[6]);
         a.d.eps = (float)eps;
-        if (!(eps >= 0) || !std::isfinite(a.d.eps)) refuse("eps must be finite and not negative");
         layout(a.x, a.d.x_sample, a.d.x_pixel);
         const auto opt = a.x.options(), f32 = opt.dtype(at::kFloat);
         at::Tensor y = at::empty(a.x.sizes(), opt), mean, rstd;
