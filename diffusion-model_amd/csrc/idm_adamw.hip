@@ -35,6 +35,7 @@ namespace {
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 constexpr int BLOCK = IDM_ADAMW_BLOCK;      // entries that share a window
 constexpr int CHUNK = 4096;                 // entries of one workgroup
+constexpr int64_t LAUNCH = (1 << 24) - 1;   // workgroups of one launch: fewer than 2^32 threads
 constexpr int TENSORS = 96;                 // tensors of one launch (their table travels in the kernel arguments, at most 4 KB)
 constexpr uint32_t ROT_A = 0xC13FA9A9u, ROT_B = 0x91E10DA5u;
 
@@ -254,21 +255,21 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t *__res
                                                             const int16_t *__restrict__ m_base, const int16_t *__restrict__ v_base,
                                                             float *__restrict__ m_out, float *__restrict__ v_out, int64_t n)
 {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    const uint32_t cm = *(const uint32_t *)(m + i), cv = *(const uint32_t *)(v + i);
-    const int bm = m_base[i / BLOCK], bv = v_base[i / BLOCK];
-    f32x4 a, b;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+        const uint32_t cm = *(const uint32_t *)(m + i), cv = *(const uint32_t *)(v + i);
+        const int bm = m_base[i / BLOCK], bv = v_base[i / BLOCK];
+        f32x4 a, b;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        a[j] = value_m(cm >> 8 * j & 255u, bm);
-        b[j] = value_v(cv >> 8 * j & 255u, bv);
+        for (int j = 0; j < 4; ++j) {
+            a[j] = value_m(cm >> 8 * j & 255u, bm);
+            b[j] = value_v(cv >> 8 * j & 255u, bv);
+        }
+        *(f32x4 *)(m_out + i) = a;
+        *(f32x4 *)(v_out + i) = b;
     }
-    *(f32x4 *)(m_out + i) = a;
-    *(f32x4 *)(v_out + i) = b;
 }
 
-template <bool EIGHT, typename F> int by_types(int pt, int gt, F &&f)
+template <typename F> int by_types(int pt, int gt, F &&f)
 {
     auto with_g = [&](auto p) {
         switch (gt) {
@@ -311,7 +312,7 @@ try {
     };
     const size_t pb = cfg->param_dtype == IDM_DT_F32 ? 4 : 2, gb = cfg->grad_dtype == IDM_DT_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {
-        if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 40)) return idm_set_error(IDM_ERR_INVALID, "adamw: tensor size out of range");
+        if (sizes[i] < 0 || sizes[i] > LAUNCH * CHUNK) return idm_set_error(IDM_ERR_INVALID, "adamw: tensor size out of range");
         if (!(weight_decay[i] >= 0) || std::isinf(weight_decay[i]))
             return idm_set_error(IDM_ERR_INVALID, "adamw: weight decay must be finite and not negative");
         total += room_of(sizes[i]);
@@ -368,30 +369,26 @@ try {
                                v_dev, m_base_dev, v_base_dev);
             return IDM_OK;
         };
-        by_types<true>(cfg->param_dtype, cfg->grad_dtype, go);
+        by_types(cfg->param_dtype, cfg->grad_dtype, go);
         tab.count = 0;
         chunks = 0;
         return hipGetLastError() == hipSuccess ? IDM_OK : idm_set_error(IDM_ERR_HIP, "adamw: launch failed");
     };
     for (int64_t i = 0; i < n_tensors; at += room_of(sizes[i]), ++i) {
         if (!sizes[i] || !grads_dev[i]) continue;      // no gradient: the tensor and its moments stay as they are
-        // a tensor of more chunks than one launch has workgroups is cut
-        const int64_t most = (int64_t)1 << 28;
-        for (int64_t lo = 0; lo < sizes[i]; lo += most * CHUNK) {
-            const int64_t n = std::min<int64_t>(sizes[i] - lo, most * CHUNK), c = (n + CHUNK - 1) / CHUNK;
-            if (tab.count == TENSORS || chunks + c > 0x7fffffff) {
-                const int rc = flush();
-                if (rc != IDM_OK) return rc;
-            }
-            const int k = tab.count++;
-            tab.p[k] = (char *)params_dev[i] + lo * pb;
-            tab.g[k] = (const char *)grads_dev[i] + lo * gb;
-            tab.n[k] = n;
-            tab.at[k] = (uint32_t)((at + lo) / BLOCK);
-            tab.first[k] = (int32_t)chunks;
-            tab.keep[k] = (float)(1.0 - cfg->lr * (double)weight_decay[i]);
-            chunks += c;
+        const int64_t c = (sizes[i] + CHUNK - 1) / CHUNK;
+        if (tab.count == TENSORS || chunks + c > LAUNCH) {
+            const int rc = flush();
+            if (rc != IDM_OK) return rc;
         }
+        const int k = tab.count++;
+        tab.p[k] = params_dev[i];
+        tab.g[k] = grads_dev[i];
+        tab.n[k] = sizes[i];
+        tab.at[k] = (uint32_t)(at / BLOCK);
+        tab.first[k] = (int32_t)chunks;
+        tab.keep[k] = (float)(1.0 - cfg->lr * (double)weight_decay[i]);
+        chunks += c;
     }
     return flush();
 } catch (...) {   // the table of memory spans is the only thing that can throw
@@ -414,7 +411,8 @@ int idm_adamw_moments(int device, const uint8_t *m_dev, const uint8_t *v_dev, co
             if ((uintptr_t)at[i] < (uintptr_t)at[k] + bytes[k] && (uintptr_t)at[k] < (uintptr_t)at[i] + bytes[i])
                 return idm_set_error(IDM_ERR_INVALID, "adamw: the moments' values share memory with their codes or each other");
     if (hipSetDevice(device) != hipSuccess) return idm_set_error(IDM_ERR_HIP, "adamw: no such device");
-    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)((moments / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, m_dev, v_dev,
+    const int64_t blocks = std::min<int64_t>((moments + 1023) / 1024, 1 << 20);   // (one pass up to 2^30 entries)
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, m_dev, v_dev,
                        m_base_dev, v_base_dev, m_out_dev, v_out_dev, moments);
     return hipGetLastError() == hipSuccess ? IDM_OK : idm_set_error(IDM_ERR_HIP, "adamw: launch failed");
 }

@@ -44,3 +44,14 @@ def test_bases_that_are_not_aligned_are_refused():
     for bases in ((MB + 1, VB), (MB, VB + 3)):
         rc, why = step(bases=bases)
         assert rc == -1 and b"aligned" in why
+
+
+def test_a_tensor_that_one_launch_cannot_cover_is_refused():
+    """(2^24 - 1) workgroups of 256 threads and 4 096 entries: fewer than 2^32 threads."""
+    most = ((1 << 24) - 1) * 4096
+    at = dict(params=(1 << 45, PARAM), grads=(1 << 46, GRAD), m=1 << 47, v=1 << 48, bases=(1 << 49, 1 << 50))
+    for n in (most + 1, 1 << 36, 1 << 40):
+        rc, why = step(sizes=(n, 20), **at)
+        assert rc == -1 and b"size" in why, (n, rc, why)
+    rc, why = step(sizes=(most, 20), bases=(MB, MB), **{k: a for k, a in at.items() if k != "bases"})
+    assert rc == -1 and b"share" in why, (rc, why)      # (as far as the next check)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from isingdiff import AdamW, adamw_state, adamw_step
+from isingdiff import AdamW, adamw_moments, adamw_state, adamw_step
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,21 @@ def test_an_eps_below_the_normal_float32_numbers(eps, bits):
         adamw_step([q], [g], r, eps=2.0 ** -100, weight_decay=0.0)
         assert torch.equal(p[1::2], before[1::2])
     assert torch.equal(p, q) and all(torch.equal(s[k], r[k]) for k in s)
+
+
+def test_more_moments_than_one_pass_of_the_grid():
+    """2^30 entries are decoded in one pass, the 768 behind them in a second."""
+    n = (1 << 30) + 768
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB of GPU memory")
+    s = {"step": torch.zeros(1, dtype=torch.int64, device="cuda")}
+    for k in "mv":
+        s[k] = torch.randint(0, 256, (n,), dtype=torch.uint8, device="cuda")
+        s[k + "_base"] = torch.randint(0, 1500, (n // 256,), dtype=torch.int16, device="cuda")
+    m, v = adamw_moments(s)
+    for lo in (0, (1 << 29) - 512, (1 << 30) - 1024):     # each part by itself gives the same
+        part = slice(lo, lo + 1792), slice(lo // 256, lo // 256 + 7)
+        few = {k: t[part[k.endswith("base")]].clone() for k, t in s.items() if k != "step"}
+        a, b = adamw_moments({**few, "step": s["step"]})
+        assert torch.equal(a, m[part[0]]) and torch.equal(b, v[part[0]])
+    assert int((v == 0).sum()) == int((s["v"] == 0).sum()) and int((m == 0).sum()) == int((s["m"] & 127 == 0).sum())
