@@ -325,8 +325,8 @@ struct State {
     void *at(int k) const { return t[k].defined() ? t[k].mutable_data_ptr() : nullptr; }
 };
 
-// A state that fits `total` entries (-1: any whole number of blocks) on `dev` (null: where it is)
-State state_of(PyObject *dict, int64_t total, const c10::Device *dev)
+// The tensors of a state, as they are
+State state_of(PyObject *dict)
 {
     State s;
     const auto take = [&](int k) {
@@ -342,6 +342,12 @@ State state_of(PyObject *dict, int64_t total, const c10::Device *dev)
     for (int k : {STEP, V}) take(k);
     if (s.eight)
         for (int k : {M_BASE, V_BASE}) take(k);
+    return s;
+}
+
+// Refuses a state that does not fit `total` entries (-1: any whole number of blocks) on `dev` (null: where it is)
+void check_state(const State &s, int64_t total, const c10::Device *dev)
+{
     const c10::Device on = dev ? *dev : s.t[M].device();
     if (total < 0) total = s.t[M].numel() / BLOCK * BLOCK;
     for (int k = 0; k < (s.eight ? 5 : 3); ++k) {
@@ -353,7 +359,6 @@ State state_of(PyObject *dict, int64_t total, const c10::Device *dev)
                    on.str() + ": make it with adamw_state for these parameters");
     }
     if (total && s.at(M) == s.at(V)) refuse("state['m'] and state['v'] are the same memory");
-    return s;
 }
 
 struct Items {   // of any iterable: references of its own, so that nothing that runs meanwhile can drop them
@@ -375,15 +380,32 @@ PyObject *adamw_step(PyObject *, PyObject *const *arg, Py_ssize_t)
         const int64_t n = params.size();
         if (!n || n != grads.size()) refuse("params and grads must be lists of the same length, not empty");
         if (betas.size() != 2) refuse("betas must be two numbers");
+        // numbers and state first: asking for them may run anybody's code, and no tensor changes any more once it has been looked at
+        std::vector<float> decay(n);
+        idm_adamw_cfg cfg = {};
+        if (PyFloat_Check(arg[6]) || PyLong_Check(arg[6])) {
+            std::fill(decay.begin(), decay.end(), (float)number(arg[6]));
+        } else {
+            const Items each(arg[6]);
+            if (each.size() != n) refuse("weight_decay must be a number or one per tensor");
+            for (int64_t i = 0; i < n; ++i) decay[i] = (float)number(each[i]);
+        }
+        cfg.lr = number(arg[3]);
+        cfg.beta1 = number(betas[0]);
+        cfg.beta2 = number(betas[1]);
+        cfg.eps = number(arg[5]);
+        bool fine = std::isfinite(cfg.lr) && cfg.lr >= 0 && std::isfinite(cfg.eps) && cfg.eps >= 0 && cfg.beta1 >= 0 && cfg.beta1 < 1 &&
+                    cfg.beta2 >= 0 && cfg.beta2 < 1;
+        for (const float d : decay) fine = fine && d >= 0 && std::isfinite(d);
+        if (!fine) refuse("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)");
+        const State s = state_of(arg[2]);
         std::vector<at::Tensor> keep;              // dense copies of gradients, until the launch
         std::vector<const at::Tensor *> changed;
         std::vector<void *> param_at(n);
         std::vector<const void *> grad_at(n);
         std::vector<int64_t> sizes(n);
-        std::vector<float> decay(n);
         changed.reserve(n);
         int64_t total = 0;
-        idm_adamw_cfg cfg = {};
         const at::Tensor *first = nullptr, *first_grad = nullptr;
         for (int64_t i = 0; i < n; ++i) {
             if (!THPVariable_Check(params[i])) refuse("params must be a list of tensors");
@@ -412,23 +434,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *arg, Py_ssize_t)
             changed.push_back(&p);
         }
         if (!first_grad) cfg.grad_dtype = cfg.param_dtype;
-        if (PyFloat_Check(arg[6]) || PyLong_Check(arg[6])) {
-            std::fill(decay.begin(), decay.end(), (float)number(arg[6]));
-        } else {
-            const Items each(arg[6]);
-            if (each.size() != n) refuse("weight_decay must be a number or one per tensor");
-            for (int64_t i = 0; i < n; ++i) decay[i] = (float)number(each[i]);
-        }
-        cfg.lr = number(arg[3]);
-        cfg.beta1 = number(betas[0]);
-        cfg.beta2 = number(betas[1]);
-        cfg.eps = number(arg[5]);
-        bool fine = std::isfinite(cfg.lr) && cfg.lr >= 0 && std::isfinite(cfg.eps) && cfg.eps >= 0 && cfg.beta1 >= 0 && cfg.beta1 < 1 &&
-                    cfg.beta2 >= 0 && cfg.beta2 < 1;
-        for (const float d : decay) fine = fine && d >= 0 && std::isfinite(d);
-        if (!fine) refuse("lr, eps and weight_decay must be finite and not negative, betas in [0, 1)");
         const c10::Device dev = first->device();
-        const State s = state_of(arg[2], total, &dev);
+        check_state(s, total, &dev);
         cfg.moment_bits = s.eight ? 8 : 32;
         if (!dev.is_cuda()) refuse("parameters must be CUDA tensors");
         const c10::DeviceGuard guard(dev);
@@ -458,7 +465,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *arg, Py_ssize_t)
 PyObject *adamw_moments(PyObject *, PyObject *dict)
 {
     return guarded([&]() -> PyObject * {
-        const State s = state_of(dict, -1, nullptr);
+        const State s = state_of(dict);
+        check_state(s, -1, nullptr);
         if (!s.eight) return Py_BuildValue("(NN)", THPVariable_Wrap(s.t[M]), THPVariable_Wrap(s.t[V]));
         if (!s.t[M].is_cuda()) refuse("the state must be on a CUDA device");
         const c10::DeviceGuard guard(s.t[M].device());

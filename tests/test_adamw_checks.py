@@ -3,8 +3,9 @@ before the first HIP call."""
 import ctypes as C
 
 import pytest
+import torch
 
-from isingdiff import _lib
+from isingdiff import _lib, adamw_state, adamw_step
 
 PARAM, GRAD, M, V, MB, VB, STEP, SCRATCH = (k << 20 for k in range(1, 9))
 
@@ -55,3 +56,25 @@ def test_a_tensor_that_one_launch_cannot_cover_is_refused():
         assert rc == -1 and b"size" in why, (n, rc, why)
     rc, why = step(sizes=(most, 20), bases=(MB, MB), **{k: a for k, a in at.items() if k != "bases"})
     assert rc == -1 and b"share" in why, (rc, why)      # (as far as the next check)
+
+
+def test_numbers_are_taken_before_the_tensors_are_looked_at():
+    """A number's __float__ is anybody's code: what it does to a parameter is seen by the checks."""
+    p = torch.zeros(300)
+
+    class Decay:
+        def __float__(self):
+            p.data = torch.zeros(7)
+            return 0.1
+    state = adamw_state([p])
+    with pytest.raises(ValueError, match="shape"):
+        adamw_step([p], [torch.zeros(300)], state, weight_decay=[Decay()])
+
+    class State(dict):
+        def __getitem__(self, k):
+            q.data = torch.zeros(7)
+            return super().__getitem__(k)
+    q = torch.zeros(300)
+    state = State(adamw_state([q]))
+    with pytest.raises(ValueError, match="shape"):
+        adamw_step([q], [torch.zeros(300)], state)
