@@ -383,7 +383,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *arg, Py_ssize_t)
         // numbers and state first: asking for them may run anybody's code, and no tensor changes any more once it has been looked at
         std::vector<float> decay(n);
         idm_adamw_cfg cfg = {};
-        if (PyFloat_Check(arg[6]) || PyLong_Check(arg[6])) {
+        if (PyFloat_Check(arg[6]) || PyLong_Check(arg[6]) || (PyNumber_Check(arg[6]) && !PySequence_Check(arg[6]))) {
             std::fill(decay.begin(), decay.end(), (float)number(arg[6]));
         } else {
             const Items each(arg[6]);

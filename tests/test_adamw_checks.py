@@ -2,6 +2,7 @@
 before the first HIP call."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -78,3 +79,10 @@ def test_numbers_are_taken_before_the_tensors_are_looked_at():
     state = State(adamw_state([q]))
     with pytest.raises(ValueError, match="shape"):
         adamw_step([q], [torch.zeros(300)], state)
+
+
+@pytest.mark.parametrize("decay", [np.float32(0.1), np.float64(0.1), np.int64(0), 0, True, np.array([0.1]), torch.tensor([0.1]), (0.1 for _ in range(1))])
+def test_any_number_is_a_weight_decay(decay):
+    p = torch.zeros(3)
+    with pytest.raises(ValueError, match="CUDA"):      # (as far as the device)
+        adamw_step([p], [p.clone()], adamw_state([p]), weight_decay=decay)
