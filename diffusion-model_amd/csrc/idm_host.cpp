@@ -148,6 +148,10 @@ at::Tensor optional_tensor(PyObject *o, const char *name)
 Norm norm_args(PyObject *x, PyObject *gamma, PyObject *beta, PyObject *shift, PyObject *groups, PyObject *activation)
 {
     Norm a;
+    PyObject *whole = PyNumber_Index(groups);   // (first: it may run anybody's code)
+    a.groups = whole ? PyLong_AsLongLong(whole) : 0;
+    Py_XDECREF(whole);
+    if (PyErr_Occurred()) PyErr_Clear();
     if (!THPVariable_Check(x) || THPVariable_Unpack(x).dim() < 2) refuse("x must be a tensor (B, ..., C)");
     a.x = THPVariable_Unpack(x);
     a.d.dtype = dtype_of(a.x);
@@ -158,8 +162,6 @@ Norm norm_args(PyObject *x, PyObject *gamma, PyObject *beta, PyObject *shift, Py
     else { PyErr_Clear(); refuse("activation must be 'none' or 'swish'"); }
     a.batch = a.x.size(0);
     a.channels = a.x.size(-1);
-    a.groups = PyLong_Check(groups) ? PyLong_AsLongLong(groups) : 0;
-    if (PyErr_Occurred()) PyErr_Clear();
     if (a.groups <= 0 || !a.channels || a.channels % a.groups || a.channels > (1 << 30))
         refuse("groups must divide the " + std::to_string(a.channels) + " channels");
     const int64_t b = a.batch, c = a.channels;
