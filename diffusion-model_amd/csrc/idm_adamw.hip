@@ -13,15 +13,16 @@
 // divide).  The twenty bits that are cut off are rounded with the dither (i * A + t * B mod 2^32) >> 12, A and B the golden-ratio
 // constants of two dimensions (2^32 / p, 2^32 / p^2, p^3 = p + 1; swapped for v): equidistributed over the steps of one entry,
 // so that a second moment that changes by 0.1 % a step, a hundredth of a code, moves by one code in about a hundred steps, where
-// rounding to nearest would never move it.  A second moment above zero never gets code zero.  Entries that are not finite take the
+// rounding to nearest would never move it.  A second moment of 2^-129 and more never gets code zero.  Entries that are not finite take the
 // largest code and leave their block's window to the others.
 //
 // Memory bounds it: parameter, gradient and moments are read once, parameter and moments written once, 28 bytes an entry with all of them
 // float32, 10 with 16-bit parameters and gradients and codes.  50 M entries float32: 268 us (5.2 TB/s; a large copy reaches 4.9, a sum of
-// two arrays 5.8); 100 M bf16 with codes: 215 us (4.7 TB/s; the codes' arithmetic is hidden to two thirds), their decoding 165 us (6.1 TB/s).
+// two arrays 5.8), with codes 157 (5.1 TB/s); 100 M bf16 with codes: 218 us (4.6 TB/s; the codes' arithmetic is hidden to two thirds), their
+// decoding 164 us (6.1 TB/s).
 // All tensors go in one launch for each 96: a workgroup takes 4 096 entries of one of them and finds it by bisection in a table that
 // travels with the arguments, so nothing is copied to the device first.  The step is counted and the bias corrected on the device, so
-// that a captured step goes on counting: by a kernel of one thread before a large step (2 us and a launch), within a small one.
+// that a captured step goes on counting: by a kernel of one thread before a large step (4.8 us), within a small one.
 #include "../../include/isingdiff.h"
 #include "idm_internal.h"
 #include "idm_device.h"
@@ -68,8 +69,8 @@ DEVI Coef coef_of(int64_t t, const Clock &c)
 
 // A step of one launch of at most kOnce workgroups counts itself: they all read the count, and each adds one to the bits above it when
 // it has done so; the last of them moves the count on and clears those bits.  (A negative count stays one until somebody adds, and nobody
-// who sees one adds.)  Larger steps begin with a kernel of one thread: the additions go one after the other (one workgroup 3.8 us instead
-// of 4.8 and 3 us less of host, 198 of them 8.2 and 8.5, 960 27 and 21).
+// who sees one adds.)  Larger steps begin with a kernel of one thread: the additions go one after the other (in a graph: one workgroup
+// 6.5 us instead of 7.1, 128 of them 8.1 and 8.3, 256 11.4 and 9.4, 960 29 and 22; the host takes 1 to 2 us less).
 constexpr int kOnce = 256, kCountBits = 53;
 
 __global__ void adamw_begin_kernel(Clock clock, Coef *c)
@@ -123,7 +124,8 @@ template <typename T, int N> DEVI void store_entries(T *p, int64_t i, int64_t n,
     }
 }
 
-// sqrt and 1 / x by the instructions (one unit in the last place each; the moments do not depend on them).  v_sqrt_f32 takes
+// sqrt and 1 / x by the instructions (one unit in the last place each: the update has 16 roundings of float32 in line at most; the moments
+// do not depend on them).  v_sqrt_f32 takes
 // denormals for zero, hence the scale.
 DEVI float root_of(float v)
 {

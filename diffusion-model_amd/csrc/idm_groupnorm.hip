@@ -12,11 +12,11 @@
 // no atomics: equal inputs give equal bits.
 //
 // Memory bounds both directions: x in, y out (forward), x and dy in, dx out (backward); a large copy on this card moves 4.9 TB/s.  Next
-// comes the vector unit: a value costs about 15 of its slots forward (exp and rcp are four each) and 25 backward, a third to two
-// thirds of the time of its memory.  Two forms:
+// comes the vector unit: a value costs about 18 of its slots forward (exp and rcp are four each) and 32 backward (1 024 x 14 x 14 x 192
+// bf16: 18 and 32 us), half to two thirds of the time of its memory.  Two forms:
 //   units   one launch; a workgroup holds a channel tile of one sample (or of several small ones) in registers, so memory is touched
-//           once.  Backward adds a small launch for the weight gradients.  Forward 1 024 x 28 x 28 x 96 bf16: 79 us (3.9 TB/s; 105 in
-//           chunks); 4 096 x 7 x 7 x 128 bf16 22 us (4.7 TB/s; 42); backward 1 024 x 14 x 14 x 192 bf16: 68 us (3.4 TB/s; 93).
+//           once.  Backward adds a small launch for the weight gradients.  Forward 1 024 x 28 x 28 x 96 bf16: 77-83 us (3.9 TB/s; 105 in
+//           chunks); 4 096 x 7 x 7 x 128 bf16 22 us (4.6 TB/s; 42); backward 1 024 x 14 x 14 x 192 bf16: 60-63 us and 5 of that launch (3.5 TB/s; 93).
 //   chunks  two launches over chunks of pixels: partial sums, then their join and the result; x (and dy) are read twice, the second
 //           time mostly from the caches.  For maps that a compute unit cannot hold, few large ones, and calls whose pointers, strides
 //           or channels are no multiples of 16 bytes.  4 x 128 x 128 x 64 fp16: 14 us forward; 3 x 127 x 125 x 64 fp16: 15 us backward.

@@ -3,7 +3,7 @@
 //
 // Why not in Python: an operator of a small map takes the device 6 us and a step over 66 tensors 9 us, while asking each of 66
 // parameters and gradients for its type, device, shape, strides and address through Python alone takes 40 us.  Here group_norm_forward
-// costs the host 6 us, a step over 66 tensors 9.
+// costs the host 6.5 us (few groups; the plan weighs every tile, 4 096 groups of 4 take it 30 us more each time), a step over 66 tensors 8.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

@@ -223,7 +223,9 @@ class BitflipTrainer:
     X and flips are (B,H,W) 0/1 (the noisy images, and which of their bits to flip), t the step index of each sample.  The norms
     (with the time vectors added on the way in) and the optimizer step run on this library's kernels, forward and backward; the
     convolutions are torch matrix products over gathered 3x3 neighbourhoods.  ``precision="bf16"`` computes with bfloat16
-    activations and operands; weights, statistics, moments and gradients of weights stay float32.  Kernels (``*_w``) decay, offsets
+    activations and operands (the gradients of kernels and of the offsets behind them are bfloat16 results, rounded once); weights, statistics,
+    moments and the gradients of norms and time vectors stay float32.  The optimizer is :class:`AdamW` with Keras's default epsilon, which Keras adds to the root before
+    the bias correction and AdamW after it.  Kernels (``*_w``) decay, offsets
     and scales do not."""
 
     def __init__(self, weights: dict, device: int = 0, time_step: int = 100, precision: str = "fp32", time_input: str = "float",

@@ -372,7 +372,9 @@ int idm_group_norm_workspace(const idm_group_norm_desc *d, int backward, size_t 
 
 /* u = x + shift[b, c];  xhat = (u - mean) * rstd with mean and rstd = 1 / sqrt(var + eps) over the pixels and channels of a
  * group;  y = act(xhat * gamma[c] + beta[c]).  gamma, beta, shift: float32, each may be NULL (1, 0, 0).  mean_dev, rstd_dev:
- * (batch, groups) float32, kept for the backward pass.  Arithmetic is float32; y is rounded once. */
+ * (batch, groups) float32, kept for the backward pass.  Arithmetic is float32; y is rounded once.  The variance
+ * is a sum of squared distances from the mean: rstd is 0 where that sum leaves float32 (2^128).  16-bit x without a shift may take it from sums
+ * of squares where the mean is within four deviations of zero, which loses five of the 24 bits at most. */
 int idm_group_norm_forward(int device, const idm_group_norm_desc *d, const void *x_dev, const float *gamma_dev,
                            const float *beta_dev, const float *shift_dev, void *y_dev, float *mean_dev, float *rstd_dev,
                            void *workspace_dev, size_t workspace_bytes, void *stream);
@@ -388,7 +390,7 @@ int idm_group_norm_backward(int device, const idm_group_norm_desc *d, const void
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * where an eps between 0 and 2^-126 counts as 2^-126.
  * params / grads / sizes / weight_decay: host arrays of n_tensors device pointers, entry counts and decays; a NULL gradient leaves
- * its tensor and moments as they are.  Gradients and parameters are dense.  What a step writes
+ * its tensor and moments as they are, but the count of steps, and with it the bias correction, is one for all tensors.  Gradients and parameters are dense.  What a step writes
  * (parameters, moments, bases, step count, scratch) must not share memory, nor a gradient with any of it (but for its own parameter, entry
  * by entry): such calls are refused.
  * Moments: tensor i's begin at the sum of the sizes before it, each rounded up to IDM_ADAMW_BLOCK entries; `moments` is that sum
